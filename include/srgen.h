@@ -514,6 +514,74 @@ SRGEN_API int srgen_clip_grad_norm_scratch_bytes(size_t* bytes);
 SRGEN_API int srgen_clip_grad_norm(float* grad, size_t numel, float max_norm, float* norm_coef2, void* scratch,
                                    size_t scratch_bytes, void* stream);
 
+/* ---- optimizer operators over a list of tensors ---------------------------------------------------------------------------
+ * Replaces: torch.optim.AdamW.step() (train.py:97,159,176,270,274-275), torch.nn.utils.clip_grad_norm_ (train.py:175) and
+ * the logged gradient norm (train.py:23-28) where the parameters are separate tensors -- the loops that keep their own
+ * optimizer -- and with moments in 8 bits.  Host mirror: superresolution_amd/optim.py.
+ *
+ * A list is `count` device pointers with element counts and types (SRGEN_F32, SRGEN_BF16; gradients of the norm and scale
+ * also SRGEN_F16); an address has the alignment of its element, nothing more.  The list travels in the kernel arguments, in
+ * as many launches as it needs: nothing is uploaded and nothing is kept from one call to the next, so calls may be captured
+ * into graphs.  Tensors that are written must not overlap one another.  count == 0 and empty tensors are allowed.
+ *
+ * Moments: one buffer for all tensors of a list; tensor i starts at element offset[i] (a multiple of 32, its part padded to
+ * a multiple of 32, the padding zero).
+ *   bits 32: m = first moment, v = second moment, fp32, 16-byte aligned
+ *   bits  8: m = first moment, v = SQUARE ROOT of the second, OCP e4m3 codes (4-byte aligned), and one e8m0 scale (byte e:
+ *            2^(e - 127)) for each 32 of them in m_scale / v_scale.  The scale is the smallest that keeps the block's largest
+ *            value at or under 1.75 * 2^8; moments are evaluated in 64 bits, rounded to fp32 and from there stochastically:
+ *            16 random bits are added under the last bit that is kept.  A root that is not zero is not stored as zero;
+ *            what is not finite is stored as NaN.
+ *   step: int32 step counters, one for each 4,096 elements of each tensor, tensors in order (srgen_adamw_counters): all
+ *         counters of a tensor are equal; a call adds 1 to those of the tensors that take the step
+ * Random bits come from (seed, step count, position in the moments' buffer) alone; bf16 parameters are rounded stochastically
+ * as well (fp32 ones to nearest). */
+enum { SRGEN_F16 = 2 };
+#define SRGEN_OPT_BLOCK 32
+#define SRGEN_OPT_CHUNK 4096
+
+typedef struct srgen_moments {
+    int32_t bits;             /* 32 or 8 */
+    int32_t reserved;         /* 0 */
+    void* m;
+    void* v;
+    uint8_t* m_scale;         /* 8 bits only */
+    uint8_t* v_scale;
+    int32_t* step;
+    uint64_t numel;           /* elements of m and v, a multiple of 32 */
+    uint64_t counters;        /* elements of step */
+} srgen_moments;
+
+typedef struct srgen_adamw_args {
+    double lr, beta1, beta2, eps, weight_decay;   /* lr, eps, weight_decay >= 0; 0 <= beta < 1 */
+    const float* lr_dev;      /* device scalar used instead of lr, or NULL                                     */
+    const float* grad_mul;    /* device scalar the gradients are multiplied by (clip coefficient), or NULL      */
+    const float* grad_div;    /* device scalar the gradients are divided by (loss scale), or NULL               */
+    const float* found_inf;   /* device scalar: not zero = nothing happens, no counter moves; or NULL           */
+    uint32_t seed;            /* of the stochastic rounding */
+    int32_t maximize;         /* 1: the gradients' sign is changed */
+} srgen_adamw_args;
+
+SRGEN_API int srgen_adamw_counters(int count, const uint64_t* numel, uint64_t* counters);
+/* One step of every tensor with g[i] != NULL (parameters p: SRGEN_F32 or SRGEN_BF16, gradients either). */
+SRGEN_API int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint64_t* numel, const uint64_t* offset,
+                               const int32_t* p_dtype, const int32_t* g_dtype, const srgen_moments* moments,
+                               const srgen_adamw_args* args, void* stream);
+/* norm_coef2 = {L2 norm of all tensors together, min(1, max_norm / (norm + 1e-6))}; sums in 64 bits, in a fixed order.  A NaN
+ * norm gives a NaN coefficient.  scratch: 8-byte aligned. */
+SRGEN_API int srgen_total_norm_scratch_bytes(int count, const uint64_t* numel, size_t* bytes);
+SRGEN_API int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, const int32_t* dtype, double max_norm,
+                               float* norm_coef2, void* scratch, size_t scratch_bytes, void* stream);
+/* g[i] *= *coef (device scalar), rounded to nearest; a coefficient of 1 writes nothing. */
+SRGEN_API int srgen_scale_many(int count, void* const* g, const uint64_t* numel, const int32_t* dtype, const float* coef,
+                               void* stream);
+/* fp32 moments to the 8-bit form, to nearest (values that 8 bits hold come back as they were), and back (v = root^2).
+ * m8, r8: numel rounded up to 32 bytes, 4-byte aligned; me, re: one byte for each 32.  m, v: any 4-byte aligned address. */
+SRGEN_API int srgen_moments_pack(const float* m, const float* v, size_t numel, uint8_t* m8, uint8_t* me, uint8_t* r8, uint8_t* re,
+                                 void* stream);
+SRGEN_API int srgen_moments_unpack(const uint8_t* m8, const uint8_t* me, const uint8_t* r8, const uint8_t* re, float* m, float* v,
+                                   size_t numel, void* stream);
+
 SRGEN_API const char* srgen_last_error(void);
 SRGEN_API int srgen_abi_version(void);
 

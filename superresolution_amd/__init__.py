@@ -10,6 +10,7 @@ from .functional import bilinear_resize, batch_metrics, pixel_losses, weighted_l
 from .autograd import pixel_loss  # noqa: F401
 from . import weights  # noqa: F401
 from . import data  # noqa: F401
+from . import optim  # noqa: F401
 
 __all__ = ["Generator", "ResBlock", "ChannelAttention", "UpsampleBlock", "Discriminator", "DiscBlock",
-           "RelativisticAverageLoss", "bilinear_resize", "batch_metrics", "pixel_losses", "weighted_l1", "pixel_loss", "weights", "data"]
+           "RelativisticAverageLoss", "bilinear_resize", "batch_metrics", "pixel_losses", "weighted_l1", "pixel_loss", "weights", "data", "optim"]

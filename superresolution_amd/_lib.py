@@ -10,7 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(CSRC, "libsrgen.so")
 
-SRGEN_F32, SRGEN_BF16 = 0, 1
+SRGEN_F32, SRGEN_BF16, SRGEN_F16 = 0, 1, 2
 NUM_TAPS = 11
 DISC_NUM_TAPS = 10
 TAP_NAMES = ("stem", "block0", "block7", "ca8", "block16", "ca17", "skip", "upsample", "output1",
@@ -31,6 +31,19 @@ class srgen_config(ctypes.Structure):
 
 class srdisc_config(ctypes.Structure):
     _fields_ = [("in_ch", ctypes.c_int32), ("base_ch", ctypes.c_int32)]
+
+
+class srgen_moments(ctypes.Structure):
+    _fields_ = [("bits", ctypes.c_int32), ("reserved", ctypes.c_int32), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("step", ctypes.c_void_p),
+                ("numel", ctypes.c_uint64), ("counters", ctypes.c_uint64)]
+
+
+class srgen_adamw_args(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("lr_dev", ctypes.c_void_p), ("grad_mul", ctypes.c_void_p),
+                ("grad_div", ctypes.c_void_p), ("found_inf", ctypes.c_void_p), ("seed", ctypes.c_uint32),
+                ("maximize", ctypes.c_int32)]
 
 
 def build(force: bool = False, jobs: int = 4) -> str:
@@ -175,6 +188,16 @@ def lib() -> ctypes.CDLL:
     for name in ("srgen_create", "srgen_destroy", "srgen_set_tensor", "srgen_commit_weights",
                  "srgen_workspace_bytes", "srgen_forward", "srgen_forward_taps", "srgen_forward_profile", "srgen_bilinear_resize", "srgen_normalize",
                  "srgen_metrics_scratch_bytes", "srgen_metrics"):
+        getattr(L, name).restype = i
+    L.srgen_adamw_counters.argtypes = [i, vp, ctypes.POINTER(ctypes.c_uint64)]
+    L.srgen_adamw_many.argtypes = [i, vp, vp, vp, vp, vp, vp, ctypes.POINTER(srgen_moments), ctypes.POINTER(srgen_adamw_args), vp]
+    L.srgen_total_norm_scratch_bytes.argtypes = [i, vp, psz]
+    L.srgen_total_norm.argtypes = [i, vp, vp, vp, ctypes.c_double, vp, vp, sz, vp]
+    L.srgen_scale_many.argtypes = [i, vp, vp, vp, vp, vp]
+    L.srgen_moments_pack.argtypes = [vp, vp, sz, vp, vp, vp, vp, vp]
+    L.srgen_moments_unpack.argtypes = [vp, vp, vp, vp, vp, vp, sz, vp]
+    for name in ("srgen_adamw_counters", "srgen_adamw_many", "srgen_total_norm_scratch_bytes", "srgen_total_norm",
+                 "srgen_scale_many", "srgen_moments_pack", "srgen_moments_unpack"):
         getattr(L, name).restype = i
     if L.srgen_abi_version() != 1:
         raise SrgenError(f"libsrgen.so ABI version {L.srgen_abi_version()} != 1; rebuild it")

@@ -1,0 +1,65 @@
+// srgen_optim.h -- kernel launch interface of the optimizer operators over many tensors (srgen_optim_api.cpp checks and
+// batches, srgen_optim_kernels.hip computes).  Not part of the public ABI (include/srgen.h).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace srgen {
+
+// Tensors travel to the kernels by value, in the kernel arguments (4 KiB at most): nothing is uploaded, nothing is kept
+// between calls, and a captured graph holds its own copy.
+constexpr int kOptBlock = 32;        // elements that share one power-of-two scale (8-bit moments)
+constexpr int kOptChunk = 4096;      // elements of one workgroup of the step, and of one step counter
+constexpr int kOptMaxTensors = 120;  // tensors of one launch
+
+constexpr uint64_t kNumelMask = (1ull << 48) - 1;   // numel_flags: bits 0..47 numel, 48..51 first type, 52..55 second type
+
+struct OptTensor {
+    void* p;               // parameter (step) or gradient (scale)
+    const void* g;         // gradient; NULL: this tensor takes no step
+    uint64_t numel_flags;  // see kNumelMask
+    uint32_t offset32;     // start in the moments' buffers, in blocks of 32 elements
+    uint32_t block0;       // first workgroup of this launch that works on it
+};
+struct OptTensors {
+    OptTensor t[kOptMaxTensors];
+    int count;
+    uint32_t counter0;     // step: counter of workgroup 0; norm: its partial sum
+};
+
+struct AdamWScalars {
+    double beta1, beta2, ln_beta1, ln_beta2, lr, eps, wd;
+    const float* lr_dev;
+    const float* grad_mul;
+    const float* grad_div;
+    const float* found_inf;
+    uint32_t seed_key;     // mix(seed)
+    int negate;
+};
+struct MomentPtrs {
+    void* m;               // fp32, or e4m3 codes
+    void* v;               // fp32 second moment, or e4m3 codes of its square root
+    uint8_t* m_scale;
+    uint8_t* v_scale;
+    int32_t* step;
+};
+struct AdamWArgs {
+    OptTensors ts;
+    AdamWScalars sc;
+    MomentPtrs mo;
+};
+static_assert(sizeof(AdamWArgs) <= 4096, "kernel arguments hold 4 KiB");
+
+uint32_t opt_mix(uint32_t x);        // the hash of the stochastic rounding (host side, for the seed)
+
+hipError_t launch_adamw_many(const AdamWArgs& a, int bits, uint32_t blocks, hipStream_t s);
+hipError_t launch_norm_partial(const OptTensors& ts, uint32_t blocks, uint32_t per_block, double* partial, hipStream_t s);
+hipError_t launch_norm_final(const double* partial, uint32_t n, double max_norm, float* norm_coef, hipStream_t s);
+hipError_t launch_scale_many(const OptTensors& ts, uint32_t blocks, const float* coef, hipStream_t s);
+hipError_t launch_moments_pack(const float* m, const float* v, size_t n, uint8_t* m8, uint8_t* me, uint8_t* r8, uint8_t* re,
+                               hipStream_t s);
+hipError_t launch_moments_unpack(const uint8_t* m8, const uint8_t* me, const uint8_t* r8, const uint8_t* re, float* m, float* v,
+                                 size_t n, hipStream_t s);
+
+}  // namespace srgen

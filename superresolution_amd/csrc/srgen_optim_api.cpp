@@ -1,0 +1,209 @@
+// srgen_optim_api.cpp -- C ABI of the optimizer operators over a list of tensors (include/srgen.h): argument checks, and the
+// list cut into launches whose descriptors fit the kernel arguments.
+#include "../../include/srgen.h"
+#include "srgen_internal.h"
+#include "srgen_optim.h"
+
+#include <math.h>
+
+using namespace srgen;
+
+static_assert(SRGEN_OPT_BLOCK == kOptBlock && SRGEN_OPT_CHUNK == kOptChunk, "include/srgen.h states the kernels' sizes");
+
+namespace {
+
+#define HIP_TRY(expr)                                                                      \
+    do {                                                                                   \
+        hipError_t e_ = (expr);                                                            \
+        if (e_ != hipSuccess)                                                              \
+            return fail(SRGEN_E_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), \
+                        __FILE__, __LINE__);                                               \
+    } while (0)
+
+// workgroups of 256 threads in one launch: the grid is counted in threads, in 32 bits
+constexpr uint64_t kMaxBlocks = (1ull << 24) - 1;
+
+inline size_t element_bytes(int dtype) { return dtype == SRGEN_F32 ? 4 : 2; }
+inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+inline uint64_t chunks_of(uint64_t n, uint64_t per) { return (n + per - 1) / per; }
+
+int check_list(int count, const void* const* t, const uint64_t* numel, const int32_t* dtype, const char* what, bool f16)
+{
+    if (count < 0) return fail(SRGEN_E_INVALID, "count %d", count);
+    if (count && (!t || !numel || !dtype)) return fail(SRGEN_E_INVALID, "NULL list");
+    for (int i = 0; i < count; ++i) {
+        if (numel[i] > kMaxBlocks * kOptChunk) return fail(SRGEN_E_UNSUPPORTED, "%s %d: %llu elements", what, i, (unsigned long long)numel[i]);
+        if (dtype[i] != SRGEN_F32 && dtype[i] != SRGEN_BF16 && !(f16 && dtype[i] == SRGEN_F16))
+            return fail(SRGEN_E_UNSUPPORTED, "%s %d: type %d", what, i, dtype[i]);
+        if (t[i] && !aligned(t[i], element_bytes(dtype[i]))) return fail(SRGEN_E_INVALID, "%s %d is not aligned to its element", what, i);
+    }
+    return SRGEN_OK;
+}
+
+// elements of one workgroup of the norm: more for long lists, so that the partial sums stay few enough for one workgroup to add
+uint32_t norm_per_block(int count, const uint64_t* numel)
+{
+    uint64_t total = 0;
+    for (int i = 0; i < count; ++i) total += numel[i];
+    uint64_t per = kOptChunk;
+    while (per < (1u << 20) && total / per > 8192) per *= 2;
+    return (uint32_t)per;
+}
+
+}  // namespace
+
+extern "C" {
+
+int srgen_adamw_counters(int count, const uint64_t* numel, uint64_t* counters)
+{
+    if (count < 0 || (count && !numel) || !counters) return fail(SRGEN_E_INVALID, "NULL argument or count %d", count);
+    uint64_t n = 0;
+    for (int i = 0; i < count; ++i) n += chunks_of(numel[i], kOptChunk);
+    *counters = n;
+    return SRGEN_OK;
+}
+
+int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint64_t* numel, const uint64_t* offset,
+                     const int32_t* p_dtype, const int32_t* g_dtype, const srgen_moments* mo, const srgen_adamw_args* args, void* stream)
+{
+    if (int rc = check_list(count, p, numel, p_dtype, "parameter", false)) return rc;
+    if (int rc = check_list(count, g, numel, g_dtype, "gradient", false)) return rc;
+    if (!mo || !args || (count && !offset)) return fail(SRGEN_E_INVALID, "NULL argument");
+    if (mo->bits != 8 && mo->bits != 32) return fail(SRGEN_E_UNSUPPORTED, "moments of %d bits: 8 or 32", mo->bits);
+    // (not (x >= 0): NaN is refused as well)
+    if (!(args->lr >= 0.0) || !(args->eps >= 0.0) || !(args->weight_decay >= 0.0) || !(args->beta1 >= 0.0 && args->beta1 < 1.0) ||
+        !(args->beta2 >= 0.0 && args->beta2 < 1.0))
+        return fail(SRGEN_E_INVALID, "lr %g, betas %g %g, eps %g, weight decay %g", args->lr, args->beta1, args->beta2, args->eps, args->weight_decay);
+    uint64_t counters = 0;
+    for (int i = 0; i < count; ++i) {
+        if (numel[i] && !p[i]) return fail(SRGEN_E_INVALID, "parameter %d is NULL", i);
+        if (offset[i] % kOptBlock || offset[i] / kOptBlock > 0xFFFFFFFFull) return fail(SRGEN_E_INVALID, "offset %d: %llu", i, (unsigned long long)offset[i]);
+        if (offset[i] + chunks_of(numel[i], kOptBlock) * kOptBlock > mo->numel)
+            return fail(SRGEN_E_INVALID, "the moments of tensor %d end behind their buffer", i);
+        counters += chunks_of(numel[i], kOptChunk);
+    }
+    if (counters > mo->counters) return fail(SRGEN_E_INVALID, "%llu step counters, %llu needed", (unsigned long long)mo->counters, (unsigned long long)counters);
+    if (!counters) return SRGEN_OK;
+    const size_t al = mo->bits == 32 ? 16 : 4;
+    if (!mo->m || !mo->v || !mo->step || (mo->bits == 8 && (!mo->m_scale || !mo->v_scale))) return fail(SRGEN_E_INVALID, "NULL moments");
+    if (!aligned(mo->m, al) || !aligned(mo->v, al) || !aligned(mo->step, 4)) return fail(SRGEN_E_INVALID, "misaligned moments");
+
+    AdamWArgs a;
+    a.sc = AdamWScalars{args->beta1, args->beta2, log(args->beta1), log(args->beta2), args->lr, args->eps, args->weight_decay,
+                        args->lr_dev, args->grad_mul, args->grad_div, args->found_inf, opt_mix(args->seed), args->maximize};
+    a.mo = MomentPtrs{mo->m, mo->v, mo->m_scale, mo->v_scale, mo->step};
+    uint64_t done = 0;                                     // step counters of the launches so far
+    for (int i = 0; i < count;) {
+        uint64_t blocks = 0;
+        bool any = false;
+        a.ts.count = 0;
+        for (; i < count && a.ts.count < kOptMaxTensors; ++i) {
+            const uint64_t c = chunks_of(numel[i], kOptChunk);
+            if (blocks + c > kMaxBlocks) break;
+            if (!c) continue;
+            any |= g[i] != nullptr;
+            a.ts.t[a.ts.count++] = OptTensor{p[i], g[i], numel[i] | (uint64_t)p_dtype[i] << 48 | (uint64_t)g_dtype[i] << 52,
+                                             (uint32_t)(offset[i] / kOptBlock), (uint32_t)blocks};
+            blocks += c;
+        }
+        a.ts.counter0 = (uint32_t)done;
+        done += blocks;
+        if (any) HIP_TRY(launch_adamw_many(a, mo->bits, (uint32_t)blocks, (hipStream_t)stream));
+    }
+    return SRGEN_OK;
+}
+
+int srgen_total_norm_scratch_bytes(int count, const uint64_t* numel, size_t* bytes)
+{
+    if (count < 0 || (count && !numel) || !bytes) return fail(SRGEN_E_INVALID, "NULL argument or count %d", count);
+    const uint32_t per = norm_per_block(count, numel);
+    uint64_t n = 0;
+    for (int i = 0; i < count; ++i) n += chunks_of(numel[i], per);
+    *bytes = (size_t)((n * sizeof(double) + 255) & ~(uint64_t)255);
+    return SRGEN_OK;
+}
+
+int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, const int32_t* dtype, double max_norm, float* norm_coef2,
+                     void* scratch, size_t scratch_bytes, void* stream)
+{
+    if (int rc = check_list(count, g, numel, dtype, "tensor", true)) return rc;
+    if (!norm_coef2) return fail(SRGEN_E_INVALID, "norm_coef2 is NULL");
+    const uint32_t per = norm_per_block(count, numel);
+    uint64_t total = 0;
+    for (int i = 0; i < count; ++i) {
+        if (numel[i] && !g[i]) return fail(SRGEN_E_INVALID, "tensor %d is NULL", i);
+        total += chunks_of(numel[i], per);
+    }
+    if (total > 0xFFFFFFFFull) return fail(SRGEN_E_UNSUPPORTED, "%llu partial sums", (unsigned long long)total);
+    if (total && (!scratch || !aligned(scratch, 8))) return fail(SRGEN_E_INVALID, "scratch is NULL or misaligned");
+    if (scratch_bytes < total * sizeof(double))
+        return fail(SRGEN_E_WORKSPACE, "scratch of %zu bytes, %zu needed", scratch_bytes, (size_t)total * sizeof(double));
+    OptTensors ts;
+    uint64_t done = 0;
+    for (int i = 0; i < count;) {
+        uint64_t blocks = 0;
+        ts.count = 0;
+        for (; i < count && ts.count < kOptMaxTensors; ++i) {
+            const uint64_t c = chunks_of(numel[i], per);
+            if (blocks + c > kMaxBlocks) break;
+            if (!c) continue;
+            ts.t[ts.count++] = OptTensor{nullptr, g[i], numel[i] | (uint64_t)dtype[i] << 48, 0, (uint32_t)blocks};
+            blocks += c;
+        }
+        ts.counter0 = (uint32_t)done;
+        done += blocks;
+        if (blocks) HIP_TRY(launch_norm_partial(ts, (uint32_t)blocks, per, (double*)scratch, (hipStream_t)stream));
+    }
+    HIP_TRY(launch_norm_final((const double*)scratch, (uint32_t)total, max_norm, norm_coef2, (hipStream_t)stream));
+    return SRGEN_OK;
+}
+
+int srgen_scale_many(int count, void* const* g, const uint64_t* numel, const int32_t* dtype, const float* coef, void* stream)
+{
+    if (int rc = check_list(count, g, numel, dtype, "tensor", true)) return rc;
+    if (!coef) return fail(SRGEN_E_INVALID, "coef is NULL");
+    OptTensors ts;
+    ts.counter0 = 0;
+    for (int i = 0; i < count; ++i)
+        if (numel[i] && !g[i]) return fail(SRGEN_E_INVALID, "tensor %d is NULL", i);
+    for (int i = 0; i < count;) {
+        uint64_t blocks = 0;
+        ts.count = 0;
+        for (; i < count && ts.count < kOptMaxTensors; ++i) {
+            const uint64_t c = chunks_of(numel[i], kOptChunk);
+            if (blocks + c > kMaxBlocks) break;
+            if (!c) continue;
+            ts.t[ts.count++] = OptTensor{g[i], nullptr, numel[i] | (uint64_t)dtype[i] << 48, 0, (uint32_t)blocks};
+            blocks += c;
+        }
+        if (blocks) HIP_TRY(launch_scale_many(ts, (uint32_t)blocks, coef, (hipStream_t)stream));
+    }
+    return SRGEN_OK;
+}
+
+static int check_pack(const void* m, const void* v, size_t n, const void* m8, const void* me, const void* r8, const void* re)
+{
+    if (!m || !v || !m8 || !me || !r8 || !re) return fail(SRGEN_E_INVALID, "NULL argument");
+    if (!aligned(m, 4) || !aligned(v, 4) || !aligned(m8, 4) || !aligned(r8, 4)) return fail(SRGEN_E_INVALID, "operands must be 4-byte aligned");
+    if (n > kMaxBlocks * 1024) return fail(SRGEN_E_UNSUPPORTED, "%zu elements", n);
+    return SRGEN_OK;
+}
+
+int srgen_moments_pack(const float* m, const float* v, size_t numel, uint8_t* m8, uint8_t* me, uint8_t* r8, uint8_t* re, void* stream)
+{
+    if (numel == 0) return SRGEN_OK;
+    if (int rc = check_pack(m, v, numel, m8, me, r8, re)) return rc;
+    HIP_TRY(launch_moments_pack(m, v, numel, m8, me, r8, re, (hipStream_t)stream));
+    return SRGEN_OK;
+}
+
+int srgen_moments_unpack(const uint8_t* m8, const uint8_t* me, const uint8_t* r8, const uint8_t* re, float* m, float* v, size_t numel,
+                         void* stream)
+{
+    if (numel == 0) return SRGEN_OK;
+    if (int rc = check_pack(m, v, numel, m8, me, r8, re)) return rc;
+    HIP_TRY(launch_moments_unpack(m8, me, r8, re, m, v, numel, (hipStream_t)stream));
+    return SRGEN_OK;
+}
+
+}  // extern "C"

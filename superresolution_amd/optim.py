@@ -1,0 +1,479 @@
+"""Optimizer operators over a list of tensors (include/srgen.h, "optimizer operators over a list of tensors").
+
+The reference's loops hold their parameters as separate tensors: ``optim.AdamW(generator.parameters(), lr)``
+(``train.py:270,274-275``), ``grad_norm(generator)`` (``train.py:23-28,96``) and ``clip_grad_norm_(generator.parameters(), 10)``
+(``train.py:175``).  Here those lines run as a few launches over the whole list:
+
+    from superresolution_amd import optim
+    opt_g = optim.AdamW(generator.parameters(), lr=cfg.lr_g, max_grad_norm=cfg.grad_clip_norm)   # clips inside step()
+    opt_d = optim.AdamW(discriminator.parameters(), lr=cfg.lr_d, state_bits=8)                   # moments in 8 bits
+    g = optim.grad_norm(generator)                                                               # 0-dim device tensor
+    optim.clip_grad_norm_(generator.parameters(), 10.0)
+
+``training.FlatAdamW`` (the fused training steps' optimizer) re-points the parameters at one flat buffer; nothing is re-pointed
+here, any address will do.  ROCm tensors only: there is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+from array import array
+from itertools import accumulate
+from operator import attrgetter
+from typing import List, Optional, Tuple
+
+import torch
+
+from . import _lib
+
+BLOCK = 32            # SRGEN_OPT_BLOCK: elements that share one scale (8-bit moments)
+CHUNK = 4096          # SRGEN_OPT_CHUNK: elements of one step counter
+
+_CODE = {torch.float32: _lib.SRGEN_F32, torch.bfloat16: _lib.SRGEN_BF16, torch.float16: _lib.SRGEN_F16}
+_TYPES = frozenset((torch.float32, torch.bfloat16))                  # of parameters and their gradients
+_dtype_of = attrgetter("dtype")
+_grad_of = attrgetter("grad")
+_data_ptr = torch.Tensor.data_ptr
+_numel = torch.Tensor.numel
+_is_contiguous = torch.Tensor.is_contiguous
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _up(n: int, to: int) -> int:
+    return -(-n // to) * to
+
+
+def _addr(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Every element at an address of its own and no gaps: what an elementwise kernel may walk in storage order."""
+    if t.numel() == 0:
+        return True
+    want = 1
+    for size, stride in sorted((z for z in zip(t.shape, t.stride()) if z[0] != 1), key=lambda z: z[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _one_device(tensors, what: str) -> torch.device:
+    devs = {t.device for t in tensors}
+    if len(devs) != 1 or next(iter(devs)).type != "cuda":
+        raise RuntimeError(f"{what}: tensors of one ROCm device, got {sorted(map(str, devs))}; there is no CPU fallback")
+    return next(iter(devs))
+
+
+def _no_overlap(spans, what: str) -> None:
+    """``spans``: (address, bytes) of tensors that are written."""
+    end = 0
+    for a, n in sorted(s for s in spans if s[1]):
+        if a < end:
+            raise RuntimeError(f"{what}: two of the tensors share memory (the same one twice?)")
+        end = a + n
+
+
+# ---- moments -----------------------------------------------------------------------------------------------------------
+class Moments:
+    """First and second moments of a list of tensors in one buffer each, the part of every tensor padded to whole blocks of 32
+    elements, and the step counters.  32 bits: ``exp_avg``, ``exp_avg_sq`` (fp32).  8 bits: ``exp_avg`` and ``root`` -- the
+    square root of the second moment -- in ``float8_e4m3fn``, with a ``float8_e8m0fnu`` power of two for each block in
+    ``exp_avg_scale`` / ``root_scale``.  The square root has half the second moment's range in powers of two, which is what
+    lets four bits of exponent and a scale hold it."""
+
+    def __init__(self, numels: List[int], bits: int, device: torch.device):
+        if bits not in (8, 32):
+            raise ValueError(f"moments of {bits} bits: 8 or 32")
+        self.numels, self.bits, self.device = list(numels), bits, device
+        sizes = [_up(n, BLOCK) for n in numels]
+        self.offsets = [0, *accumulate(sizes)][:-1]
+        self.total = sum(sizes)
+        counters = [-(-n // CHUNK) for n in numels]
+        self.counter0 = [0, *accumulate(counters)]
+        self.step = torch.zeros(self.counter0[-1], dtype=torch.int32, device=device)
+        if bits == 32:
+            self.exp_avg = torch.zeros(self.total, dtype=torch.float32, device=device)
+            self.exp_avg_sq = torch.zeros(self.total, dtype=torch.float32, device=device)
+            ptrs = (self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), None, None)
+        else:
+            def byte(n, value):
+                return torch.full((n,), value, dtype=torch.uint8, device=device)
+            self.exp_avg = byte(self.total, 0).view(torch.float8_e4m3fn)
+            self.root = byte(self.total, 0).view(torch.float8_e4m3fn)
+            self.exp_avg_scale = byte(self.total // BLOCK, 1).view(torch.float8_e8m0fnu)      # what zeros are packed with
+            self.root_scale = byte(self.total // BLOCK, 1).view(torch.float8_e8m0fnu)
+            ptrs = tuple(t.data_ptr() for t in (self.exp_avg, self.root, self.exp_avg_scale, self.root_scale))
+        self._numel, self._offset = array("Q", self.numels), array("Q", self.offsets)
+        self._c = _lib.srgen_moments(bits, 0, *ptrs, self.step.data_ptr(), self.total, self.counter0[-1])
+
+    @property
+    def nbytes(self) -> int:
+        """Device memory of the moments (without the step counters)."""
+        return self.total * 8 if self.bits == 32 else 2 * self.total + 2 * (self.total // BLOCK)
+
+    def steps(self) -> List[int]:
+        """Steps each tensor has taken (reads them back from the device)."""
+        if not self.numels:
+            return []
+        host = self.step.cpu()
+        return [int(host[c]) if n else 0 for c, n in zip(self.counter0, self.numels)]
+
+    def set_steps(self, steps: List[int]) -> None:
+        counts = [b - a for a, b in zip(self.counter0, self.counter0[1:])]
+        self.step.copy_(torch.repeat_interleave(torch.tensor(steps, dtype=torch.int32), torch.tensor(counts)))
+
+    def read(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Both moments as fp32 buffers in the padded layout (8 bits: new ones; 32 bits: the buffers themselves)."""
+        if self.bits == 32:
+            return self.exp_avg, self.exp_avg_sq
+        return unpack_moments(self.exp_avg, self.exp_avg_scale, self.root, self.root_scale, self.total)
+
+    def write(self, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor) -> None:
+        """Takes fp32 buffers in the padded layout (the padding has to be zero)."""
+        if self.bits == 32:
+            self.exp_avg.copy_(exp_avg)
+            self.exp_avg_sq.copy_(exp_avg_sq)
+            return
+        _pack_into(exp_avg, exp_avg_sq, self.exp_avg, self.exp_avg_scale, self.root, self.root_scale)
+
+    def update(self, p: array, g: array, p_dtype: array, g_dtype: array, args: "_lib.srgen_adamw_args", stream: int) -> None:
+        """One AdamW step of the list (addresses and type codes in the list's order; address 0: no gradient)."""
+        _lib.check(_lib.lib().srgen_adamw_many(len(self.numels), _addr(p), _addr(g), _addr(self._numel), _addr(self._offset),
+                                               _addr(p_dtype), _addr(g_dtype), self._c, args, stream))
+
+
+def _pack_into(exp_avg, exp_avg_sq, m8, me, r8, re) -> None:
+    with torch.cuda.device(exp_avg.device):
+        _lib.check(_lib.lib().srgen_moments_pack(exp_avg.data_ptr(), exp_avg_sq.data_ptr(), exp_avg.numel(), m8.data_ptr(), me.data_ptr(),
+                                                 r8.data_ptr(), re.data_ptr(), _stream(exp_avg.device)))
+
+
+def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor):
+    """``(m, m_scale, r, r_scale)``: the moments (flat fp32) as ``Moments`` holds them in 8 bits -- e4m3 values of the first
+    moment and of the second one's square root, rounded to nearest, with a power of two for each 32 elements; ``m`` and ``r``
+    are padded with zeros to whole blocks.  Values that 8 bits hold come back from ``unpack_moments`` as they were."""
+    dev = _one_device((exp_avg, exp_avg_sq), "pack_moments")
+    for t in (exp_avg, exp_avg_sq):
+        if t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous() or t.shape != exp_avg.shape:
+            raise RuntimeError(f"pack_moments: two flat contiguous fp32 tensors of one length, got {tuple(t.shape)} {t.dtype}")
+    n = _up(exp_avg.numel(), BLOCK)
+    m8, r8 = (torch.empty(n, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
+    me, re = (torch.empty(n // BLOCK, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu) for _ in range(2))
+    _pack_into(exp_avg, exp_avg_sq, m8, me, r8, re)
+    return m8, me, r8, re
+
+
+def unpack_moments(m8: torch.Tensor, m_scale: torch.Tensor, r8: torch.Tensor, r_scale: torch.Tensor, numel: int):
+    """``(exp_avg, exp_avg_sq)``: the first ``numel`` elements of 8-bit moments in fp32, the second moment squared."""
+    dev = _one_device((m8, m_scale, r8, r_scale), "unpack_moments")
+    numel = int(numel)
+    if not 0 <= numel <= m8.numel():
+        raise RuntimeError(f"unpack_moments: {numel} of {m8.numel()} elements")
+    for t, want, dt in ((m8, m8.numel(), torch.float8_e4m3fn), (r8, m8.numel(), torch.float8_e4m3fn),
+                        (m_scale, m8.numel() // BLOCK, torch.float8_e8m0fnu), (r_scale, m8.numel() // BLOCK, torch.float8_e8m0fnu)):
+        if t.dtype != dt or t.dim() != 1 or not t.is_contiguous() or t.numel() != want or m8.numel() % BLOCK:
+            raise RuntimeError(f"unpack_moments: flat contiguous e4m3 values in whole blocks of {BLOCK} and an e8m0 scale for each, "
+                               f"got {tuple(t.shape)} {t.dtype}")
+        if t.data_ptr() % 4 and dt == torch.float8_e4m3fn:
+            raise RuntimeError("unpack_moments: values must be 4-byte aligned")
+    m, v = (torch.empty(numel, dtype=torch.float32, device=dev) for _ in range(2))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().srgen_moments_unpack(m8.data_ptr(), m_scale.data_ptr(), r8.data_ptr(), r_scale.data_ptr(), m.data_ptr(),
+                                                   v.data_ptr(), numel, _stream(dev)))
+    return m, v
+
+
+# ---- total norm, clipping ----------------------------------------------------------------------------------------------
+def _tensor_list(tensors, what: str) -> List[torch.Tensor]:
+    if isinstance(tensors, torch.Tensor):
+        tensors = [tensors]
+    return list(tensors)
+
+
+def _codes(tensors, what: str) -> array:
+    try:
+        return array("i", map(_CODE.__getitem__, map(_dtype_of, tensors)))
+    except KeyError as e:
+        raise RuntimeError(f"{what}: fp32, bf16 or fp16 tensors, got {e.args[0]}") from None
+
+
+def _norm_coef(tensors: List[torch.Tensor], dev: torch.device, max_norm: float) -> torch.Tensor:
+    """Device floats {norm, clip coefficient} of contiguous (or dense) tensors."""
+    codes = _codes(tensors, "total_norm")
+    ptr, numel = array("Q", map(_data_ptr, tensors)), array("Q", map(_numel, tensors))
+    L, need = _lib.lib(), ctypes.c_size_t()
+    with torch.cuda.device(dev):
+        _lib.check(L.srgen_total_norm_scratch_bytes(len(tensors), _addr(numel), ctypes.byref(need)))
+        buf = torch.empty(need.value + 8, dtype=torch.uint8, device=dev)       # partial sums, then {norm, coefficient}
+        out = buf[need.value:].view(torch.float32)
+        _lib.check(L.srgen_total_norm(len(tensors), _addr(ptr), _addr(numel), _addr(codes), max_norm, out.data_ptr(), buf.data_ptr(),
+                                      need.value, _stream(dev)))
+    return out
+
+
+def _flat_readable(t: torch.Tensor) -> torch.Tensor:
+    if t.layout != torch.strided:
+        raise RuntimeError(f"expected strided tensors, got {t.layout}")
+    return t if t.is_contiguous() or _dense(t) else t.contiguous()
+
+
+@torch.no_grad()
+def total_norm(tensors) -> torch.Tensor:
+    """The L2 norm of all ``tensors`` (fp32, bf16, fp16) taken together, as a 0-dim fp32 device tensor
+    (``torch.nn.utils.get_total_norm``).  Sums are held in 64 bits and added in a fixed order: the result does not overflow
+    before the norm itself does, and repeats bit for bit."""
+    ts = _tensor_list(tensors, "total_norm")
+    if not ts:
+        return torch.tensor(0.0)
+    dev = _one_device(ts, "total_norm")
+    return _norm_coef([_flat_readable(t) for t in ts], dev, 1.0)[0]
+
+
+def _grads(parameters) -> List[torch.Tensor]:
+    if isinstance(parameters, torch.nn.Module):
+        parameters = parameters.parameters()
+    return [p.grad for p in _tensor_list(parameters, "parameters") if p.grad is not None]
+
+
+def grad_norm(model) -> torch.Tensor:
+    """``grad_norm(model)`` of the reference's loops (``train.py:23-28``): the L2 norm of all gradients of a module (or of an
+    iterable of parameters), as a 0-dim device tensor instead of a Python float -- no synchronisation."""
+    return total_norm(_grads(model))
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` (``train.py:175``): scales the gradients in place so that their total L2 norm is at
+    most ``max_norm``; returns the norm before.  ``AdamW(max_grad_norm=...)`` clips without the extra pass."""
+    if float(norm_type) != 2.0:
+        raise NotImplementedError(f"clip_grad_norm_: the L2 norm only, got norm_type={norm_type}")
+    grads = _grads(parameters)
+    if not grads:
+        return torch.tensor(0.0)
+    dev = _one_device(grads, "clip_grad_norm_")
+    for g in grads:
+        if g.layout != torch.strided or not (g.is_contiguous() or _dense(g)):
+            raise RuntimeError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or overlaps")
+    codes, numel = _codes(grads, "clip_grad_norm_"), array("Q", map(_numel, grads))
+    ptr = array("Q", map(_data_ptr, grads))
+    _no_overlap([(a, g.numel() * g.element_size()) for a, g in zip(ptr, grads)], "clip_grad_norm_")
+    out = _norm_coef(grads, dev, float(max_norm))
+    if error_if_nonfinite and not bool(torch.isfinite(out[0])):
+        raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To "
+                           "disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().srgen_scale_many(len(grads), _addr(ptr), _addr(numel), _addr(codes), out.data_ptr() + 4, _stream(dev)))
+    torch.autograd.graph.increment_version(grads)
+    return out[0]
+
+
+# ---- AdamW -------------------------------------------------------------------------------------------------------------
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` over separate tensors, a whole parameter group in one or a few launches.
+
+    Parameters are fp32 or bf16 on one ROCm device, gradients either; arithmetic is fp32 (moments of 8 bits: 64 bits, then
+    rounded).  Beyond torch's arguments:
+
+    ``state_bits``      32: fp32 moments.  8: both moments in 8 bits (``Moments``), 2.06 bytes a parameter instead of 8, rounded
+                        stochastically, so that a moving average goes on moving when its change is under half a step.
+    ``max_grad_norm``   clips the gradients of all groups by their total norm inside ``step`` (the gradients themselves stay as
+                        they are); the norm is left in ``last_grad_norm``.
+    ``seed``            of the stochastic rounding, which depends on it, the step and the element only.
+
+    A bf16 parameter is rounded stochastically.  ``lr`` may be a 0-dim fp32 tensor on the parameters' device: a captured step
+    then follows it.  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
+    optimizer have to stay.  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
+    gradient does not happen.  ``state_dict`` has the layout of ``torch.optim.AdamW`` with fp32 moments, whatever
+    ``state_bits``: checkpoints move between the two, and between 8 and 32 bits."""
+
+    _step_supports_amp_scaling = True
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
+                 max_grad_norm: Optional[float] = None, maximize: bool = False, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits={state_bits}: 8 or 32")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"max_grad_norm={max_grad_norm}: positive, or None")
+        self.state_bits, self.max_grad_norm, self.seed = state_bits, max_grad_norm, int(seed) & 0xFFFFFFFF
+        self.last_grad_norm: Optional[torch.Tensor] = None
+        self.moments: List[Moments] = []
+        self._spans: List = []
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        g = self.param_groups[-1]
+        try:
+            _check_hyper(g)
+            dev = _one_device([p for h in self.param_groups for p in h["params"]], "AdamW")
+            for p in g["params"]:
+                if p.dtype not in _TYPES:
+                    raise RuntimeError(f"AdamW: fp32 or bf16 parameters, got {p.dtype}")
+                if not _dense(p):
+                    raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()} has gaps or overlaps")
+            if len({id(p) for p in g["params"]}) != len(g["params"]):
+                raise ValueError("AdamW: a parameter appears twice in a group")
+            _no_overlap([(p.data_ptr(), p.numel() * p.element_size()) for h in self.param_groups for p in h["params"]], "AdamW")
+        except Exception:
+            self.param_groups.pop()
+            raise
+        # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
+        self.moments.append(Moments([p.numel() for p in g["params"]], self.state_bits, dev))
+        self._spans.append(None)
+
+    # -- one step -----------------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = [self._collect(k) for k in range(len(self.param_groups))]
+        used = [g for w in work for g in w[1] if g is not None]
+        if not used:
+            return loss
+        dev = self.moments[0].device
+        if any(g.device != dev for g in used):
+            raise RuntimeError(f"AdamW: gradients on {dev}, as the parameters")
+        mul = None
+        if self.max_grad_norm is not None:
+            mul = _norm_coef(used, dev, float(self.max_grad_norm))
+            self.last_grad_norm = mul[0]
+        div, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        if mul is not None and div is not None:
+            raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
+                               "scaler.step(optimizer)")
+        for t in (div, found):
+            if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != 1):
+                raise RuntimeError(f"AdamW: grad_scale and found_inf are fp32 scalars on {dev}")
+        with torch.cuda.device(dev):
+            stream = _stream(dev)
+            for group, mo, (params, grads, ptr, p_code) in zip(self.param_groups, self.moments, work):
+                if not any(g is not None for g in grads):
+                    continue
+                lr, (b1, b2) = group["lr"], group["betas"]
+                lr_dev = None
+                if isinstance(lr, torch.Tensor):
+                    if lr.is_cuda:
+                        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
+                            raise RuntimeError(f"AdamW: a learning rate on the device is an fp32 scalar on {dev}")
+                        lr_dev, lr = lr.data_ptr(), 0.0
+                    else:
+                        lr = float(lr)
+                args = _lib.srgen_adamw_args(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev,
+                                             mul.data_ptr() + 4 if mul is not None else None, div.data_ptr() if div is not None else None,
+                                             found.data_ptr() if found is not None else None, self.seed, 1 if group["maximize"] else 0)
+                g_ptr = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+                g_code = array("i", [0 if g is None else _CODE[g.dtype] for g in grads])
+                mo.update(ptr, g_ptr, p_code, g_code, args, stream)
+                # the kernel wrote behind torch's back: the version counters are what the Generator / Discriminator mirrors
+                # watch to upload their weights again
+                torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+        return loss
+
+    def _collect(self, k: int):
+        """(parameters, gradients laid out as they are, addresses, type codes) of group ``k``, checked."""
+        params, mo = self.param_groups[k]["params"], self.moments[k]
+        ptr = array("Q", map(_data_ptr, params))
+        if list(map(_numel, params)) != mo.numels:
+            raise RuntimeError("AdamW: a parameter has another number of elements than when it was added")
+        if not _TYPES.issuperset(map(_dtype_of, params)):
+            raise RuntimeError(f"AdamW: fp32 or bf16 parameters, got {set(map(_dtype_of, params))}")
+        p_code = _codes(params, "AdamW")
+        if ptr != self._spans[k]:
+            # (addresses seen for the first time: the check is of these addresses alone)
+            self._spans[k] = ptr
+            every = [p for h in self.param_groups for p in h["params"]]
+            if _one_device(every, "AdamW") != mo.device:
+                raise RuntimeError(f"AdamW: the parameters have left {mo.device}, where their moments are")
+            _no_overlap([(p.data_ptr(), p.numel() * p.element_size()) for p in every], "AdamW")
+        grads = list(map(_grad_of, params))
+        some = [g for g in grads if g is not None]
+        if not _TYPES.issuperset(map(_dtype_of, some)):
+            raise RuntimeError(f"AdamW: fp32 or bf16 gradients, got {set(map(_dtype_of, some))}")
+        if not (all(map(_is_contiguous, some)) and all(map(_is_contiguous, params))):
+            grads = [g if g is None else self._like(p, g) for p, g in zip(params, grads)]
+        return params, grads, ptr, p_code
+
+    @staticmethod
+    def _like(p: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
+        """``g`` with its elements in the order of ``p``'s memory."""
+        if g.layout != torch.strided:
+            raise RuntimeError(f"AdamW: strided gradients, got {g.layout}")
+        if not _dense(p):
+            raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()} has gaps or overlaps")
+        if all(a == b or n == 1 for n, a, b in zip(p.shape, p.stride(), g.stride())) or (p.is_contiguous() and g.is_contiguous()):
+            return g
+        return torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=g.device).copy_(g)
+
+    # -- checkpoints --------------------------------------------------------------------------------------------------
+    def state_dict(self) -> dict:
+        """``torch.optim.AdamW.state_dict()``'s layout (``train.py:219-225`` saves it): fp32 moments and a step for each
+        parameter that has taken one.  Reads the step counts back: one synchronisation."""
+        state, groups, first = {}, [], 0
+        for group, mo in zip(self.param_groups, self.moments):
+            m, v = mo.read()
+            for i, (p, t) in enumerate(zip(group["params"], mo.steps())):
+                if t == 0:
+                    continue
+                a, n = mo.offsets[i], mo.numels[i]
+                state[first + i] = {"step": torch.tensor(float(t)), **{
+                    key: torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=mo.device).copy_(
+                        torch.as_strided(x, p.shape, p.stride(), a)) for key, x in (("exp_avg", m), ("exp_avg_sq", v))}}
+            groups.append({**{k: x for k, x in group.items() if k != "params"}, "params": list(range(first, first + len(group["params"])))})
+            first += len(group["params"])
+        return {"state": state, "param_groups": groups}
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict: dict) -> None:
+        """Takes what ``state_dict`` (of this class, whatever its ``state_bits``, of ``torch.optim.AdamW`` or of
+        ``training.FlatAdamW``) returns."""
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("loaded state dict contains a parameter group that doesn't match the size of optimizer's group")
+        state = state_dict["state"]
+        if any(g.get("amsgrad") for g in groups):
+            raise ValueError("AdamW: no amsgrad variant")
+        for group, saved in zip(self.param_groups, groups):
+            for i, (p, key) in enumerate(zip(group["params"], saved["params"])):
+                for name in ("exp_avg", "exp_avg_sq"):
+                    if key in state and state[key][name].numel() != p.numel():
+                        raise ValueError(f"optimizer state of parameter {key} has {state[key][name].numel()} entries, the parameter {p.numel()}")
+            _check_hyper({**group, **{k: x for k, x in saved.items() if k != "params"}})
+        for group, mo, saved in zip(self.param_groups, self.moments, groups):
+            m = torch.zeros(mo.total, dtype=torch.float32, device=mo.device)
+            v = torch.zeros_like(m)
+            steps = []
+            for i, (p, key) in enumerate(zip(group["params"], saved["params"])):
+                st = state.get(key)
+                steps.append(0 if st is None else int(float(st["step"])))
+                if st is not None:
+                    for x, name in ((m, "exp_avg"), (v, "exp_avg_sq")):
+                        torch.as_strided(x, p.shape, p.stride(), mo.offsets[i]).copy_(st[name].reshape(p.shape))
+            if steps:
+                mo.set_steps(steps)
+            mo.write(m, v)
+            group.update({k: x for k, x in saved.items() if k != "params"})
+
+    def __getstate__(self):
+        raise RuntimeError("AdamW holds device buffers: save state_dict() instead of the optimizer")
+
+
+def _check_hyper(g: dict) -> None:
+    b1, b2 = g["betas"]
+    if isinstance(g["lr"], torch.Tensor):
+        if g["lr"].numel() != 1:
+            raise ValueError("Tensor lr must be 1-element")
+    elif not g["lr"] >= 0.0:
+        raise ValueError(f"Invalid learning rate: {g['lr']}")
+    if not g["eps"] >= 0.0:
+        raise ValueError(f"Invalid epsilon value: {g['eps']}")
+    if not g["weight_decay"] >= 0.0:
+        raise ValueError(f"Invalid weight_decay value: {g['weight_decay']}")
+    for i, b in enumerate((b1, b2)):
+        if not 0.0 <= b < 1.0:
+            raise ValueError(f"Invalid beta parameter at index {i}: {b}")
