@@ -568,7 +568,7 @@ SRGEN_API int srgen_adamw_many(int count, void* const* p, const void* const* g, 
                                const int32_t* p_dtype, const int32_t* g_dtype, const srgen_moments* moments,
                                const srgen_adamw_args* args, void* stream);
 /* norm_coef2 = {L2 norm of all tensors together, min(1, max_norm / (norm + 1e-6))}; sums in 64 bits, in a fixed order.  A NaN
- * norm gives a NaN coefficient.  scratch: 8-byte aligned. */
+ * norm gives a NaN coefficient.  Tensors with g[i] == NULL are left out.  scratch: 8-byte aligned. */
 SRGEN_API int srgen_total_norm_scratch_bytes(int count, const uint64_t* numel, size_t* bytes);
 SRGEN_API int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, const int32_t* dtype, double max_norm,
                                float* norm_coef2, void* scratch, size_t scratch_bytes, void* stream);

@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
@@ -48,7 +49,7 @@ class srgen_adamw_args(ctypes.Structure):
 
 def build(force: bool = False, jobs: int = 4) -> str:
     """Compile the gfx950 kernels + C ABI in-tree (hipcc cross-compiles without a GPU)."""
-    cmd = ["make", "-C", CSRC, f"-j{jobs}", "libsrgen.so"]
+    cmd = ["make", "-C", CSRC, f"-j{jobs}", f"PYTHON={sys.executable}", "libsrgen.so", "../_tensorlist.so"]
     if force:
         cmd.insert(1, "-B")
     subprocess.check_call(cmd)

@@ -130,10 +130,7 @@ int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, con
     if (!norm_coef2) return fail(SRGEN_E_INVALID, "norm_coef2 is NULL");
     const uint32_t per = norm_per_block(count, numel);
     uint64_t total = 0;
-    for (int i = 0; i < count; ++i) {
-        if (numel[i] && !g[i]) return fail(SRGEN_E_INVALID, "tensor %d is NULL", i);
-        total += chunks_of(numel[i], per);
-    }
+    for (int i = 0; i < count; ++i) total += g[i] ? chunks_of(numel[i], per) : 0;
     if (total > 0xFFFFFFFFull) return fail(SRGEN_E_UNSUPPORTED, "%llu partial sums", (unsigned long long)total);
     if (total && (!scratch || !aligned(scratch, 8))) return fail(SRGEN_E_INVALID, "scratch is NULL or misaligned");
     if (scratch_bytes < total * sizeof(double))
@@ -144,7 +141,7 @@ int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, con
         uint64_t blocks = 0;
         ts.count = 0;
         for (; i < count && ts.count < kOptMaxTensors; ++i) {
-            const uint64_t c = chunks_of(numel[i], per);
+            const uint64_t c = g[i] ? chunks_of(numel[i], per) : 0;
             if (blocks + c > kMaxBlocks) break;
             if (!c) continue;
             ts.t[ts.count++] = OptTensor{nullptr, g[i], numel[i] | (uint64_t)dtype[i] << 48, 0, (uint32_t)blocks};

@@ -1,0 +1,159 @@
+// tensorlist.cpp -- Python extension `superresolution_amd._tensorlist`: addresses, sizes and types of a list of tensors.
+//
+// The optimizer operators take a list of some hundred tensors in one or two launches of a few microseconds each; asking every
+// tensor for its address, type, size and layout from Python takes ten times that (0.1 us a question).  These loops ask the
+// tensors directly.  Nothing is computed here, and nothing is kept.
+#include <Python.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ATen.h>
+
+#include <cstdint>
+
+namespace {
+
+// a writable buffer of `n` items of `size` bytes (array.array), or an exception
+struct Buffer {
+    Py_buffer b{};
+    bool ok = false;
+    Buffer(PyObject* o, Py_ssize_t n, Py_ssize_t size)
+    {
+        if (PyObject_GetBuffer(o, &b, PyBUF_WRITABLE) != 0) return;
+        if (b.len < n * size) {
+            PyErr_Format(PyExc_ValueError, "buffer of %zd bytes, %zd needed", b.len, n * size);
+            PyBuffer_Release(&b);
+            return;
+        }
+        ok = true;
+    }
+    ~Buffer()
+    {
+        if (ok) PyBuffer_Release(&b);
+    }
+    template <typename T>
+    T* as() const
+    {
+        return static_cast<T*>(b.buf);
+    }
+};
+
+int type_code(const at::Tensor& t)            // SRGEN_F32, SRGEN_BF16, SRGEN_F16
+{
+    switch (t.scalar_type()) {
+        case at::kFloat: return 0;
+        case at::kBFloat16: return 1;
+        case at::kHalf: return 2;
+        default: return -1;
+    }
+}
+
+// strided, contiguous, on the device, of a known type: what a kernel may walk from its first address
+bool plain(const at::Tensor& t, int device, int max_code, int* code)
+{
+    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device) return false;
+    *code = type_code(t);
+    return *code >= 0 && *code <= max_code && t.is_contiguous();
+}
+
+PyObject* guarded(PyObject* (*f)(PyObject*), PyObject* args)
+{
+    try {
+        return f(args);
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// params(list, device, numel, p, p_code, g, g_code) -> number of gradients, or -1: some tensor wants a closer look (another
+// type, device, size or order; the caller finds out which and says so)
+PyObject* params_impl(PyObject* args)
+{
+    PyObject *list, *o[5];
+    int device;
+    if (!PyArg_ParseTuple(args, "O!iOOOOO", &PyList_Type, &list, &device, &o[0], &o[1], &o[2], &o[3], &o[4])) return nullptr;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    Buffer numel(o[0], n, 8), p(o[1], n, 8), pc(o[2], n, 4), g(o[3], n, 8), gc(o[4], n, 4);
+    if (!numel.ok || !p.ok || !pc.ok || !g.ok || !gc.ok) return nullptr;
+    long grads = 0;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* x = PyList_GET_ITEM(list, i);
+        if (!THPVariable_Check(x)) return PyLong_FromLong(-1);
+        const at::Tensor& t = THPVariable_Unpack(x);
+        int code;
+        if (!plain(t, device, 1, &code) || (uint64_t)t.numel() != numel.as<uint64_t>()[i]) return PyLong_FromLong(-1);
+        p.as<uint64_t>()[i] = (uint64_t)(uintptr_t)t.data_ptr();
+        pc.as<int32_t>()[i] = code;
+        const at::Tensor& d = t.grad();
+        g.as<uint64_t>()[i] = 0;
+        gc.as<int32_t>()[i] = 0;
+        if (!d.defined()) continue;
+        if (!plain(d, device, 1, &code) || d.numel() != t.numel()) return PyLong_FromLong(-1);
+        g.as<uint64_t>()[i] = (uint64_t)(uintptr_t)d.data_ptr();
+        gc.as<int32_t>()[i] = code;
+        ++grads;
+    }
+    return PyLong_FromLong(grads);
+}
+
+// tensors(list, device, ptr, numel, code) -> True, or False: some tensor wants a closer look
+PyObject* tensors_impl(PyObject* args)
+{
+    PyObject *list, *o[3];
+    int device;
+    if (!PyArg_ParseTuple(args, "O!iOOO", &PyList_Type, &list, &device, &o[0], &o[1], &o[2])) return nullptr;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    Buffer ptr(o[0], n, 8), numel(o[1], n, 8), code(o[2], n, 4);
+    if (!ptr.ok || !numel.ok || !code.ok) return nullptr;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* x = PyList_GET_ITEM(list, i);
+        int c;
+        if (!THPVariable_Check(x)) Py_RETURN_FALSE;
+        const at::Tensor& t = THPVariable_Unpack(x);
+        if (!plain(t, device, 2, &c)) Py_RETURN_FALSE;
+        ptr.as<uint64_t>()[i] = (uint64_t)(uintptr_t)t.data_ptr();
+        numel.as<uint64_t>()[i] = (uint64_t)t.numel();
+        code.as<int32_t>()[i] = c;
+    }
+    Py_RETURN_TRUE;
+}
+
+// bump(list, g): version counters of the tensors that were written (those with g[i] != 0; g = None: all)
+PyObject* bump_impl(PyObject* args)
+{
+    PyObject *list, *og;
+    if (!PyArg_ParseTuple(args, "O!O", &PyList_Type, &list, &og)) return nullptr;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    const uint64_t* g = nullptr;
+    Py_buffer b{};
+    if (og != Py_None) {
+        if (PyObject_GetBuffer(og, &b, PyBUF_SIMPLE) != 0) return nullptr;
+        if (b.len < n * 8) {
+            PyBuffer_Release(&b);
+            PyErr_SetString(PyExc_ValueError, "buffer too small");
+            return nullptr;
+        }
+        g = static_cast<const uint64_t*>(b.buf);
+    }
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* x = PyList_GET_ITEM(list, i);
+        if ((g && !g[i]) || !THPVariable_Check(x)) continue;
+        const at::Tensor& t = THPVariable_Unpack(x);
+        if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    if (g) PyBuffer_Release(&b);
+    Py_RETURN_NONE;
+}
+
+PyObject* params(PyObject*, PyObject* args) { return guarded(params_impl, args); }
+PyObject* tensors(PyObject*, PyObject* args) { return guarded(tensors_impl, args); }
+PyObject* bump(PyObject*, PyObject* args) { return guarded(bump_impl, args); }
+
+PyMethodDef methods[] = {{"params", params, METH_VARARGS, "addresses and types of parameters and their gradients"},
+                         {"tensors", tensors, METH_VARARGS, "addresses, sizes and types of tensors"},
+                         {"bump", bump, METH_VARARGS, "version counters of written tensors"},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__tensorlist() { return PyModule_Create(&module); }

@@ -15,7 +15,9 @@ here, any address will do.  ROCm tensors only: there is no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import os
 from array import array
 from itertools import accumulate
 from operator import attrgetter
@@ -25,20 +27,29 @@ import torch
 
 from . import _lib
 
+try:
+    from . import _tensorlist
+except ImportError as e:
+    raise _lib.SrgenError(f"{os.path.join(os.path.dirname(_lib.CSRC), '_tensorlist.so')} is missing or does not fit the installed torch "
+                          f"({e}): run `python -c 'import __graft_entry__ as g; g.build()'`. There is no fallback path.") from e
+
 BLOCK = 32            # SRGEN_OPT_BLOCK: elements that share one scale (8-bit moments)
 CHUNK = 4096          # SRGEN_OPT_CHUNK: elements of one step counter
 
 _CODE = {torch.float32: _lib.SRGEN_F32, torch.bfloat16: _lib.SRGEN_BF16, torch.float16: _lib.SRGEN_F16}
 _TYPES = frozenset((torch.float32, torch.bfloat16))                  # of parameters and their gradients
 _dtype_of = attrgetter("dtype")
-_grad_of = attrgetter("grad")
 _data_ptr = torch.Tensor.data_ptr
 _numel = torch.Tensor.numel
-_is_contiguous = torch.Tensor.is_contiguous
 
 
 def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _on(dev: torch.device):
+    """``dev`` as the current device, for a launch."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _up(n: int, to: int) -> int:
@@ -147,7 +158,7 @@ class Moments:
 
 
 def _pack_into(exp_avg, exp_avg_sq, m8, me, r8, re) -> None:
-    with torch.cuda.device(exp_avg.device):
+    with _on(exp_avg.device):
         _lib.check(_lib.lib().srgen_moments_pack(exp_avg.data_ptr(), exp_avg_sq.data_ptr(), exp_avg.numel(), m8.data_ptr(), me.data_ptr(),
                                                  r8.data_ptr(), re.data_ptr(), _stream(exp_avg.device)))
 
@@ -181,17 +192,15 @@ def unpack_moments(m8: torch.Tensor, m_scale: torch.Tensor, r8: torch.Tensor, r_
         if t.data_ptr() % 4 and dt == torch.float8_e4m3fn:
             raise RuntimeError("unpack_moments: values must be 4-byte aligned")
     m, v = (torch.empty(numel, dtype=torch.float32, device=dev) for _ in range(2))
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.check(_lib.lib().srgen_moments_unpack(m8.data_ptr(), m_scale.data_ptr(), r8.data_ptr(), r_scale.data_ptr(), m.data_ptr(),
                                                    v.data_ptr(), numel, _stream(dev)))
     return m, v
 
 
 # ---- total norm, clipping ----------------------------------------------------------------------------------------------
-def _tensor_list(tensors, what: str) -> List[torch.Tensor]:
-    if isinstance(tensors, torch.Tensor):
-        tensors = [tensors]
-    return list(tensors)
+def _tensor_list(tensors) -> List[torch.Tensor]:
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
 
 
 def _codes(tensors, what: str) -> array:
@@ -201,24 +210,37 @@ def _codes(tensors, what: str) -> array:
         raise RuntimeError(f"{what}: fp32, bf16 or fp16 tensors, got {e.args[0]}") from None
 
 
-def _norm_coef(tensors: List[torch.Tensor], dev: torch.device, max_norm: float) -> torch.Tensor:
-    """Device floats {norm, clip coefficient} of contiguous (or dense) tensors."""
-    codes = _codes(tensors, "total_norm")
-    ptr, numel = array("Q", map(_data_ptr, tensors)), array("Q", map(_numel, tensors))
+def _arrays(n: int):
+    return array("Q", bytes(8 * n)), array("Q", bytes(8 * n)), array("i", bytes(4 * n))
+
+
+def _listed(tensors: List[torch.Tensor], what: str):
+    """(device, tensors, addresses, sizes, type codes); a tensor with gaps is taken as a contiguous copy."""
+    if not tensors[0].is_cuda:
+        _one_device(tensors, what)                                             # (raises)
+    dev = tensors[0].device
+    ptr, numel, code = _arrays(len(tensors))
+    if not _tensorlist.tensors(tensors, dev.index, ptr, numel, code):
+        _one_device(tensors, what)
+        for t in tensors:
+            if t.layout != torch.strided:
+                raise RuntimeError(f"{what}: strided tensors, got {t.layout}")
+        code = _codes(tensors, what)
+        tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
+        ptr, numel = array("Q", map(_data_ptr, tensors)), array("Q", map(_numel, tensors))
+    return dev, tensors, ptr, numel, code
+
+
+def _norm_coef(dev: torch.device, ptr: array, numel: array, code: array, max_norm: float) -> torch.Tensor:
+    """Device floats {norm, clip coefficient}; address 0: left out."""
     L, need = _lib.lib(), ctypes.c_size_t()
-    with torch.cuda.device(dev):
-        _lib.check(L.srgen_total_norm_scratch_bytes(len(tensors), _addr(numel), ctypes.byref(need)))
-        buf = torch.empty(need.value + 8, dtype=torch.uint8, device=dev)       # partial sums, then {norm, coefficient}
-        out = buf[need.value:].view(torch.float32)
-        _lib.check(L.srgen_total_norm(len(tensors), _addr(ptr), _addr(numel), _addr(codes), max_norm, out.data_ptr(), buf.data_ptr(),
+    _lib.check(L.srgen_total_norm_scratch_bytes(len(ptr), _addr(numel), need))
+    words = need.value // 4
+    buf = torch.empty(words + 2, dtype=torch.float32, device=dev)              # partial sums, then {norm, coefficient}
+    with _on(dev):
+        _lib.check(L.srgen_total_norm(len(ptr), _addr(ptr), _addr(numel), _addr(code), max_norm, buf.data_ptr() + need.value, buf.data_ptr(),
                                       need.value, _stream(dev)))
-    return out
-
-
-def _flat_readable(t: torch.Tensor) -> torch.Tensor:
-    if t.layout != torch.strided:
-        raise RuntimeError(f"expected strided tensors, got {t.layout}")
-    return t if t.is_contiguous() or _dense(t) else t.contiguous()
+    return buf[words:]
 
 
 @torch.no_grad()
@@ -226,17 +248,17 @@ def total_norm(tensors) -> torch.Tensor:
     """The L2 norm of all ``tensors`` (fp32, bf16, fp16) taken together, as a 0-dim fp32 device tensor
     (``torch.nn.utils.get_total_norm``).  Sums are held in 64 bits and added in a fixed order: the result does not overflow
     before the norm itself does, and repeats bit for bit."""
-    ts = _tensor_list(tensors, "total_norm")
+    ts = _tensor_list(tensors)
     if not ts:
         return torch.tensor(0.0)
-    dev = _one_device(ts, "total_norm")
-    return _norm_coef([_flat_readable(t) for t in ts], dev, 1.0)[0]
+    dev, ts, ptr, numel, code = _listed(ts, "total_norm")
+    return _norm_coef(dev, ptr, numel, code, 1.0)[0]
 
 
 def _grads(parameters) -> List[torch.Tensor]:
     if isinstance(parameters, torch.nn.Module):
         parameters = parameters.parameters()
-    return [p.grad for p in _tensor_list(parameters, "parameters") if p.grad is not None]
+    return [g for g in (p.grad for p in _tensor_list(parameters)) if g is not None]
 
 
 def grad_norm(model) -> torch.Tensor:
@@ -254,24 +276,42 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     grads = _grads(parameters)
     if not grads:
         return torch.tensor(0.0)
-    dev = _one_device(grads, "clip_grad_norm_")
-    for g in grads:
-        if g.layout != torch.strided or not (g.is_contiguous() or _dense(g)):
+    dev, listed, ptr, numel, code = _listed(grads, "clip_grad_norm_")
+    for g, t in zip(grads, listed):
+        if g is not t:
             raise RuntimeError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or overlaps")
-    codes, numel = _codes(grads, "clip_grad_norm_"), array("Q", map(_numel, grads))
-    ptr = array("Q", map(_data_ptr, grads))
-    _no_overlap([(a, g.numel() * g.element_size()) for a, g in zip(ptr, grads)], "clip_grad_norm_")
-    out = _norm_coef(grads, dev, float(max_norm))
+    _no_overlap([(a, n * (4 if c == _lib.SRGEN_F32 else 2)) for a, n, c in zip(ptr, numel, code)], "clip_grad_norm_")
+    out = _norm_coef(dev, ptr, numel, code, float(max_norm))
     if error_if_nonfinite and not bool(torch.isfinite(out[0])):
         raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To "
                            "disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().srgen_scale_many(len(grads), _addr(ptr), _addr(numel), _addr(codes), out.data_ptr() + 4, _stream(dev)))
-    torch.autograd.graph.increment_version(grads)
+    with _on(dev):
+        _lib.check(_lib.lib().srgen_scale_many(len(grads), _addr(ptr), _addr(numel), _addr(code), out.data_ptr() + 4, _stream(dev)))
+    _tensorlist.bump(grads, None)
     return out[0]
 
 
 # ---- AdamW -------------------------------------------------------------------------------------------------------------
+class _Lists:
+    """A group's addresses and type codes, as the kernels' list wants them; filled anew at every step."""
+
+    def __init__(self, n: int):
+        self.p, self.g, self.p_code = _arrays(n)
+        self.g_code = array("i", self.p_code)
+        self.checked = (array("Q"), array("i"))            # parameters' addresses and types that were last found apart
+
+
+def _in_order_of(p: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
+    """``g`` with its elements in the order of ``p``'s memory."""
+    if g.layout != torch.strided:
+        raise RuntimeError(f"AdamW: strided gradients, got {g.layout}")
+    if not _dense(p):
+        raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()} has gaps or overlaps")
+    if all(a == b or n == 1 for n, a, b in zip(p.shape, p.stride(), g.stride())) or (p.is_contiguous() and g.is_contiguous()):
+        return g
+    return torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=g.device).copy_(g)
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` over separate tensors, a whole parameter group in one or a few launches.
 
@@ -301,7 +341,7 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.seed = state_bits, max_grad_norm, int(seed) & 0xFFFFFFFF
         self.last_grad_norm: Optional[torch.Tensor] = None
         self.moments: List[Moments] = []
-        self._spans: List = []
+        self._lists: List[_Lists] = []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
 
     def add_param_group(self, param_group) -> None:
@@ -323,7 +363,7 @@ class AdamW(torch.optim.Optimizer):
             raise
         # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
         self.moments.append(Moments([p.numel() for p in g["params"]], self.state_bits, dev))
-        self._spans.append(None)
+        self._lists.append(_Lists(len(g["params"])))
 
     # -- one step -----------------------------------------------------------------------------------------------------
     @torch.no_grad()
@@ -332,28 +372,39 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = [self._collect(k) for k in range(len(self.param_groups))]
-        used = [g for w in work for g in w[1] if g is not None]
-        if not used:
+        counts, kept = [], []
+        for k, (group, mo, ls) in enumerate(zip(self.param_groups, self.moments, self._lists)):
+            n = _tensorlist.params(group["params"], mo.device.index, mo._numel, ls.p, ls.p_code, ls.g, ls.g_code)
+            if n < 0:
+                n = self._look_closer(k, kept)
+            if ls.p != ls.checked[0] or ls.p_code != ls.checked[1]:
+                self._check_memory()
+            counts.append(n)
+        if not any(counts):
             return loss
         dev = self.moments[0].device
-        if any(g.device != dev for g in used):
-            raise RuntimeError(f"AdamW: gradients on {dev}, as the parameters")
-        mul = None
+        norm_coef = None
         if self.max_grad_norm is not None:
-            mul = _norm_coef(used, dev, float(self.max_grad_norm))
-            self.last_grad_norm = mul[0]
+            if len(counts) == 1:
+                ls = self._lists[0]
+                g, numel, code = ls.g, self.moments[0]._numel, ls.g_code
+            else:
+                g, numel, code = array("Q"), array("Q"), array("i")
+                for mo, ls in zip(self.moments, self._lists):
+                    g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
+            norm_coef = _norm_coef(dev, g, numel, code, float(self.max_grad_norm))
+            self.last_grad_norm = norm_coef[0]
         div, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
-        if mul is not None and div is not None:
+        if norm_coef is not None and div is not None:
             raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
                                "scaler.step(optimizer)")
         for t in (div, found):
             if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != 1):
                 raise RuntimeError(f"AdamW: grad_scale and found_inf are fp32 scalars on {dev}")
-        with torch.cuda.device(dev):
+        with _on(dev):
             stream = _stream(dev)
-            for group, mo, (params, grads, ptr, p_code) in zip(self.param_groups, self.moments, work):
-                if not any(g is not None for g in grads):
+            for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
+                if not n:
                     continue
                 lr, (b1, b2) = group["lr"], group["betas"]
                 lr_dev = None
@@ -365,50 +416,40 @@ class AdamW(torch.optim.Optimizer):
                     else:
                         lr = float(lr)
                 args = _lib.srgen_adamw_args(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev,
-                                             mul.data_ptr() + 4 if mul is not None else None, div.data_ptr() if div is not None else None,
-                                             found.data_ptr() if found is not None else None, self.seed, 1 if group["maximize"] else 0)
-                g_ptr = array("Q", [0 if g is None else g.data_ptr() for g in grads])
-                g_code = array("i", [0 if g is None else _CODE[g.dtype] for g in grads])
-                mo.update(ptr, g_ptr, p_code, g_code, args, stream)
+                                             None if norm_coef is None else norm_coef.data_ptr() + 4, None if div is None else div.data_ptr(),
+                                             None if found is None else found.data_ptr(), self.seed, 1 if group["maximize"] else 0)
+                mo.update(ls.p, ls.g, ls.p_code, ls.g_code, args, stream)
                 # the kernel wrote behind torch's back: the version counters are what the Generator / Discriminator mirrors
                 # watch to upload their weights again
-                torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+                _tensorlist.bump(group["params"], ls.g)
         return loss
 
-    def _collect(self, k: int):
-        """(parameters, gradients laid out as they are, addresses, type codes) of group ``k``, checked."""
-        params, mo = self.param_groups[k]["params"], self.moments[k]
-        ptr = array("Q", map(_data_ptr, params))
+    def _look_closer(self, k: int, kept: list) -> int:
+        """Group ``k`` has a tensor that is not plain (contiguous fp32 or bf16, on the device, of the size it was added with):
+        refused, or its gradient brought into the parameter's order; such copies are put into ``kept``."""
+        params, mo, ls = self.param_groups[k]["params"], self.moments[k], self._lists[k]
         if list(map(_numel, params)) != mo.numels:
             raise RuntimeError("AdamW: a parameter has another number of elements than when it was added")
-        if not _TYPES.issuperset(map(_dtype_of, params)):
-            raise RuntimeError(f"AdamW: fp32 or bf16 parameters, got {set(map(_dtype_of, params))}")
-        p_code = _codes(params, "AdamW")
-        if ptr != self._spans[k]:
-            # (addresses seen for the first time: the check is of these addresses alone)
-            self._spans[k] = ptr
-            every = [p for h in self.param_groups for p in h["params"]]
-            if _one_device(every, "AdamW") != mo.device:
-                raise RuntimeError(f"AdamW: the parameters have left {mo.device}, where their moments are")
-            _no_overlap([(p.data_ptr(), p.numel() * p.element_size()) for p in every], "AdamW")
-        grads = list(map(_grad_of, params))
+        grads = [p.grad for p in params]
         some = [g for g in grads if g is not None]
-        if not _TYPES.issuperset(map(_dtype_of, some)):
-            raise RuntimeError(f"AdamW: fp32 or bf16 gradients, got {set(map(_dtype_of, some))}")
-        if not (all(map(_is_contiguous, some)) and all(map(_is_contiguous, params))):
-            grads = [g if g is None else self._like(p, g) for p, g in zip(params, grads)]
-        return params, grads, ptr, p_code
+        for what, ts in (("parameters", params), ("gradients", some)):
+            if not _TYPES.issuperset(map(_dtype_of, ts)):
+                raise RuntimeError(f"AdamW: fp32 or bf16 {what}, got {sorted({str(t.dtype) for t in ts})}")
+            if any(t.device != mo.device for t in ts):
+                raise RuntimeError(f"AdamW: {what} that are not on {mo.device}, where the moments are")
+        grads = [g if g is None else _in_order_of(p, g) for p, g in zip(params, grads)]
+        kept += grads
+        ls.p[:] = array("Q", map(_data_ptr, params))
+        ls.p_code[:] = _codes(params, "AdamW")
+        ls.g[:] = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+        ls.g_code[:] = array("i", [0 if g is None else _CODE[g.dtype] for g in grads])
+        return len(some)
 
-    @staticmethod
-    def _like(p: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
-        """``g`` with its elements in the order of ``p``'s memory."""
-        if g.layout != torch.strided:
-            raise RuntimeError(f"AdamW: strided gradients, got {g.layout}")
-        if not _dense(p):
-            raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()} has gaps or overlaps")
-        if all(a == b or n == 1 for n, a, b in zip(p.shape, p.stride(), g.stride())) or (p.is_contiguous() and g.is_contiguous()):
-            return g
-        return torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=g.device).copy_(g)
+    def _check_memory(self) -> None:
+        """No two parameters share memory: looked at when their addresses are not those that were looked at last."""
+        _no_overlap([(p.data_ptr(), p.numel() * p.element_size()) for h in self.param_groups for p in h["params"]], "AdamW")
+        for h, ls in zip(self.param_groups, self._lists):
+            ls.checked = array("Q", map(_data_ptr, h["params"])), _codes(h["params"], "AdamW")
 
     # -- checkpoints --------------------------------------------------------------------------------------------------
     def state_dict(self) -> dict:

@@ -91,7 +91,6 @@ def test_norm_scale_pack_refuse():
     assert L.srgen_total_norm(1, ad(p), ad(n), ad(d), 1.0, 64, None, 256, None) == -1             # no scratch
     assert L.srgen_total_norm(1, ad(p), ad(n), ad(d), 1.0, 64, 260, 256, None) == -1              # misaligned scratch
     assert L.srgen_total_norm(1, ad(p), ad(n), ad(d), 1.0, 64, 256, 8, None) == -5                # too small
-    assert L.srgen_total_norm(1, ad(array("Q", [0])), ad(n), ad(d), 1.0, 64, 256, 256, None) == -1
     assert L.srgen_total_norm(1, ad(p), ad(n), ad(array("i", [3])), 1.0, 64, 256, 256, None) == -6
     assert L.srgen_scale_many(1, ad(p), ad(n), ad(d), None, None) == -1
     assert L.srgen_scale_many(1, ad(array("Q", [4097])), ad(n), ad(array("i", [2])), 64, None) == -1
