@@ -532,8 +532,10 @@ SRGEN_API int srgen_clip_grad_norm(float* grad, size_t numel, float max_norm, fl
  *            value at or under 1.75 * 2^8; moments are evaluated in 64 bits, rounded to fp32 and from there stochastically:
  *            16 random bits are added under the last bit that is kept.  A root that is not zero is not stored as zero;
  *            what is not finite is stored as NaN.
- *   step: int32 step counters, one for each 4,096 elements of each tensor, tensors in order (srgen_adamw_counters): all
- *         counters of a tensor are equal; a call adds 1 to those of the tensors that take the step
+ *   step: int32 step counters, one for each chunk of 4,096 elements of each tensor, tensors in order
+ *         (srgen_adamw_chunk_count): all counters of a tensor are equal; a call adds 1 to those of the tensors that take the step
+ *   table: which chunk is where, four words for each, as srgen_adamw_chunk_table writes it for the list's sizes and offsets;
+ *         made once and copied to the device by the caller
  * Random bits come from (seed, step count, position in the moments' buffer) alone; bf16 parameters are rounded stochastically
  * as well (fp32 ones to nearest). */
 enum { SRGEN_F16 = 2 };
@@ -548,8 +550,9 @@ typedef struct srgen_moments {
     uint8_t* m_scale;         /* 8 bits only */
     uint8_t* v_scale;
     int32_t* step;
+    const uint32_t* table;    /* 16-byte aligned */
     uint64_t numel;           /* elements of m and v, a multiple of 32 */
-    uint64_t counters;        /* elements of step */
+    uint64_t chunks;          /* elements of step, and a quarter of the table's */
 } srgen_moments;
 
 typedef struct srgen_adamw_args {
@@ -562,7 +565,9 @@ typedef struct srgen_adamw_args {
     int32_t maximize;         /* 1: the gradients' sign is changed */
 } srgen_adamw_args;
 
-SRGEN_API int srgen_adamw_counters(int count, const uint64_t* numel, uint64_t* counters);
+SRGEN_API int srgen_adamw_chunk_count(int count, const uint64_t* numel, uint64_t* chunks);
+SRGEN_API int srgen_adamw_chunk_table(int count, const uint64_t* numel, const uint64_t* offset, uint32_t* host_table,
+                                      uint64_t chunks);
 /* One step of every tensor with g[i] != NULL (parameters p: SRGEN_F32 or SRGEN_BF16, gradients either). */
 SRGEN_API int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint64_t* numel, const uint64_t* offset,
                                const int32_t* p_dtype, const int32_t* g_dtype, const srgen_moments* moments,

@@ -37,7 +37,7 @@ class srdisc_config(ctypes.Structure):
 class srgen_moments(ctypes.Structure):
     _fields_ = [("bits", ctypes.c_int32), ("reserved", ctypes.c_int32), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
                 ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("step", ctypes.c_void_p),
-                ("numel", ctypes.c_uint64), ("counters", ctypes.c_uint64)]
+                ("table", ctypes.c_void_p), ("numel", ctypes.c_uint64), ("chunks", ctypes.c_uint64)]
 
 
 class srgen_adamw_args(ctypes.Structure):
@@ -190,14 +190,15 @@ def lib() -> ctypes.CDLL:
                  "srgen_workspace_bytes", "srgen_forward", "srgen_forward_taps", "srgen_forward_profile", "srgen_bilinear_resize", "srgen_normalize",
                  "srgen_metrics_scratch_bytes", "srgen_metrics"):
         getattr(L, name).restype = i
-    L.srgen_adamw_counters.argtypes = [i, vp, ctypes.POINTER(ctypes.c_uint64)]
+    L.srgen_adamw_chunk_count.argtypes = [i, vp, ctypes.POINTER(ctypes.c_uint64)]
+    L.srgen_adamw_chunk_table.argtypes = [i, vp, vp, vp, ctypes.c_uint64]
     L.srgen_adamw_many.argtypes = [i, vp, vp, vp, vp, vp, vp, ctypes.POINTER(srgen_moments), ctypes.POINTER(srgen_adamw_args), vp]
     L.srgen_total_norm_scratch_bytes.argtypes = [i, vp, psz]
     L.srgen_total_norm.argtypes = [i, vp, vp, vp, ctypes.c_double, vp, vp, sz, vp]
     L.srgen_scale_many.argtypes = [i, vp, vp, vp, vp, vp]
     L.srgen_moments_pack.argtypes = [vp, vp, sz, vp, vp, vp, vp, vp]
     L.srgen_moments_unpack.argtypes = [vp, vp, vp, vp, vp, vp, sz, vp]
-    for name in ("srgen_adamw_counters", "srgen_adamw_many", "srgen_total_norm_scratch_bytes", "srgen_total_norm",
+    for name in ("srgen_adamw_chunk_count", "srgen_adamw_chunk_table", "srgen_adamw_many", "srgen_total_norm_scratch_bytes", "srgen_total_norm",
                  "srgen_scale_many", "srgen_moments_pack", "srgen_moments_unpack"):
         getattr(L, name).restype = i
     if L.srgen_abi_version() != 1:

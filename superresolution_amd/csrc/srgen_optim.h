@@ -8,24 +8,19 @@
 namespace srgen {
 
 // Tensors travel to the kernels by value, in the kernel arguments (4 KiB at most): nothing is uploaded, nothing is kept
-// between calls, and a captured graph holds its own copy.
+// between calls, and a captured graph holds its own copy.  An address has 48 bits; what is above holds the element type
+// (and, where the list has no table of chunks, the upper bits of the size).
 constexpr int kOptBlock = 32;        // elements that share one power-of-two scale (8-bit moments)
 constexpr int kOptChunk = 4096;      // elements of one workgroup of the step, and of one step counter
-constexpr int kOptMaxTensors = 120;  // tensors of one launch
+constexpr int kOptMaxTensors = 240;  // tensors of one launch
+constexpr uint64_t kAddrMask = (1ull << 48) - 1;
 
-constexpr uint64_t kNumelMask = (1ull << 48) - 1;   // numel_flags: bits 0..47 numel, 48..51 first type, 52..55 second type
-
-struct OptTensor {
-    void* p;               // parameter (step) or gradient (scale)
-    const void* g;         // gradient; NULL: this tensor takes no step
-    uint64_t numel_flags;  // see kNumelMask
+// One chunk of a list that takes steps (the table is made once for a list: it depends on the sizes alone).
+struct OptChunk {
+    uint32_t tensor;       // in the list
+    uint32_t index;        // of the chunk in its tensor
     uint32_t offset32;     // start in the moments' buffers, in blocks of 32 elements
-    uint32_t block0;       // first workgroup of this launch that works on it
-};
-struct OptTensors {
-    OptTensor t[kOptMaxTensors];
-    int count;
-    uint32_t counter0;     // step: counter of workgroup 0; norm: its partial sum
+    uint32_t count;        // elements, 1 .. kOptChunk
 };
 
 struct AdamWScalars {
@@ -43,13 +38,30 @@ struct MomentPtrs {
     uint8_t* m_scale;
     uint8_t* v_scale;
     int32_t* step;
+    const OptChunk* chunks;
 };
 struct AdamWArgs {
-    OptTensors ts;
+    uint64_t p[kOptMaxTensors];   // address | type << 48
+    uint64_t g[kOptMaxTensors];   // the same; 0: the tensor takes no step
+    uint32_t tensor0;             // the list's tensor that p[0], g[0] are of
+    uint32_t chunk0;              // chunk (and step counter) of workgroup 0
     AdamWScalars sc;
     MomentPtrs mo;
 };
 static_assert(sizeof(AdamWArgs) <= 4096, "kernel arguments hold 4 KiB");
+
+// a list without a table
+struct OptTensor {
+    uint64_t ptr;          // address | type << 48 | upper 12 bits of the size << 52
+    uint32_t numel_lo;
+    uint32_t block0;       // first workgroup of this launch that works on it
+};
+struct OptTensors {
+    OptTensor t[kOptMaxTensors];
+    int count;
+    uint32_t partial0;     // norm: partial sum of workgroup 0
+};
+static_assert(sizeof(OptTensors) <= 4096 - 64, "kernel arguments hold 4 KiB");
 
 uint32_t opt_mix(uint32_t x);        // the hash of the stochastic rounding (host side, for the seed)
 

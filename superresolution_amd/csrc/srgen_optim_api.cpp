@@ -8,6 +8,7 @@
 
 using namespace srgen;
 
+static_assert(sizeof(OptChunk) == 16, "a table entry is four words");
 static_assert(SRGEN_OPT_BLOCK == kOptBlock && SRGEN_OPT_CHUNK == kOptChunk, "include/srgen.h states the kernels' sizes");
 
 namespace {
@@ -35,9 +36,15 @@ int check_list(int count, const void* const* t, const uint64_t* numel, const int
         if (numel[i] > kMaxBlocks * kOptChunk) return fail(SRGEN_E_UNSUPPORTED, "%s %d: %llu elements", what, i, (unsigned long long)numel[i]);
         if (dtype[i] != SRGEN_F32 && dtype[i] != SRGEN_BF16 && !(f16 && dtype[i] == SRGEN_F16))
             return fail(SRGEN_E_UNSUPPORTED, "%s %d: type %d", what, i, dtype[i]);
+        if ((uintptr_t)t[i] > kAddrMask) return fail(SRGEN_E_UNSUPPORTED, "%s %d: an address of more than 48 bits", what, i);
         if (t[i] && !aligned(t[i], element_bytes(dtype[i]))) return fail(SRGEN_E_INVALID, "%s %d is not aligned to its element", what, i);
     }
     return SRGEN_OK;
+}
+
+inline OptTensor list_entry(const void* t, uint64_t numel, int32_t dtype, uint64_t block0)
+{
+    return OptTensor{(uint64_t)(uintptr_t)t | (uint64_t)dtype << 48 | (numel >> 32) << 52, (uint32_t)numel, (uint32_t)block0};
 }
 
 // elements of one workgroup of the norm: more for long lists, so that the partial sums stay few enough for one workgroup to add
@@ -54,12 +61,31 @@ uint32_t norm_per_block(int count, const uint64_t* numel)
 
 extern "C" {
 
-int srgen_adamw_counters(int count, const uint64_t* numel, uint64_t* counters)
+int srgen_adamw_chunk_count(int count, const uint64_t* numel, uint64_t* chunks)
 {
-    if (count < 0 || (count && !numel) || !counters) return fail(SRGEN_E_INVALID, "NULL argument or count %d", count);
+    if (count < 0 || (count && !numel) || !chunks) return fail(SRGEN_E_INVALID, "NULL argument or count %d", count);
     uint64_t n = 0;
     for (int i = 0; i < count; ++i) n += chunks_of(numel[i], kOptChunk);
-    *counters = n;
+    *chunks = n;
+    return SRGEN_OK;
+}
+
+int srgen_adamw_chunk_table(int count, const uint64_t* numel, const uint64_t* offset, uint32_t* host_table, uint64_t chunks)
+{
+    if (count < 0 || (count && (!numel || !offset)) || (chunks && !host_table)) return fail(SRGEN_E_INVALID, "NULL argument or count %d", count);
+    uint64_t k = 0;
+    for (int i = 0; i < count; ++i) {
+        const uint64_t c = chunks_of(numel[i], kOptChunk);
+        if (offset[i] % kOptBlock || (offset[i] + numel[i]) / kOptBlock > 0xFFFFFFFEull) return fail(SRGEN_E_INVALID, "offset %d: %llu", i, (unsigned long long)offset[i]);
+        if (k + c > chunks) return fail(SRGEN_E_INVALID, "a table of %llu chunks is too short", (unsigned long long)chunks);
+        for (uint64_t x = 0; x < c; ++x, ++k) {
+            const uint64_t rest = numel[i] - x * kOptChunk;
+            host_table[4 * k] = (uint32_t)i;
+            host_table[4 * k + 1] = (uint32_t)x;
+            host_table[4 * k + 2] = (uint32_t)(offset[i] / kOptBlock + x * (kOptChunk / kOptBlock));
+            host_table[4 * k + 3] = (uint32_t)(rest < (uint64_t)kOptChunk ? rest : kOptChunk);
+        }
+    }
     return SRGEN_OK;
 }
 
@@ -74,39 +100,39 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
     if (!(args->lr >= 0.0) || !(args->eps >= 0.0) || !(args->weight_decay >= 0.0) || !(args->beta1 >= 0.0 && args->beta1 < 1.0) ||
         !(args->beta2 >= 0.0 && args->beta2 < 1.0))
         return fail(SRGEN_E_INVALID, "lr %g, betas %g %g, eps %g, weight decay %g", args->lr, args->beta1, args->beta2, args->eps, args->weight_decay);
-    uint64_t counters = 0;
+    uint64_t chunks = 0;
     for (int i = 0; i < count; ++i) {
         if (numel[i] && !p[i]) return fail(SRGEN_E_INVALID, "parameter %d is NULL", i);
         if (offset[i] % kOptBlock || offset[i] / kOptBlock > 0xFFFFFFFFull) return fail(SRGEN_E_INVALID, "offset %d: %llu", i, (unsigned long long)offset[i]);
         if (offset[i] + chunks_of(numel[i], kOptBlock) * kOptBlock > mo->numel)
             return fail(SRGEN_E_INVALID, "the moments of tensor %d end behind their buffer", i);
-        counters += chunks_of(numel[i], kOptChunk);
+        chunks += chunks_of(numel[i], kOptChunk);
     }
-    if (counters > mo->counters) return fail(SRGEN_E_INVALID, "%llu step counters, %llu needed", (unsigned long long)mo->counters, (unsigned long long)counters);
-    if (!counters) return SRGEN_OK;
+    if (chunks != mo->chunks) return fail(SRGEN_E_INVALID, "moments of %llu chunks, the list has %llu", (unsigned long long)mo->chunks, (unsigned long long)chunks);
+    if (!chunks) return SRGEN_OK;
     const size_t al = mo->bits == 32 ? 16 : 4;
-    if (!mo->m || !mo->v || !mo->step || (mo->bits == 8 && (!mo->m_scale || !mo->v_scale))) return fail(SRGEN_E_INVALID, "NULL moments");
-    if (!aligned(mo->m, al) || !aligned(mo->v, al) || !aligned(mo->step, 4)) return fail(SRGEN_E_INVALID, "misaligned moments");
+    if (!mo->m || !mo->v || !mo->step || !mo->table || (mo->bits == 8 && (!mo->m_scale || !mo->v_scale))) return fail(SRGEN_E_INVALID, "NULL moments");
+    if (!aligned(mo->m, al) || !aligned(mo->v, al) || !aligned(mo->step, 4) || !aligned(mo->table, 16)) return fail(SRGEN_E_INVALID, "misaligned moments");
 
     AdamWArgs a;
     a.sc = AdamWScalars{args->beta1, args->beta2, log(args->beta1), log(args->beta2), args->lr, args->eps, args->weight_decay,
                         args->lr_dev, args->grad_mul, args->grad_div, args->found_inf, opt_mix(args->seed), args->maximize};
-    a.mo = MomentPtrs{mo->m, mo->v, mo->m_scale, mo->v_scale, mo->step};
-    uint64_t done = 0;                                     // step counters of the launches so far
+    a.mo = MomentPtrs{mo->m, mo->v, mo->m_scale, mo->v_scale, mo->step, reinterpret_cast<const OptChunk*>(mo->table)};
+    uint64_t done = 0;                                     // chunks of the launches so far
     for (int i = 0; i < count;) {
         uint64_t blocks = 0;
+        int k = 0;
         bool any = false;
-        a.ts.count = 0;
-        for (; i < count && a.ts.count < kOptMaxTensors; ++i) {
+        a.tensor0 = (uint32_t)i;
+        for (; i < count && k < kOptMaxTensors; ++i, ++k) {
             const uint64_t c = chunks_of(numel[i], kOptChunk);
             if (blocks + c > kMaxBlocks) break;
-            if (!c) continue;
-            any |= g[i] != nullptr;
-            a.ts.t[a.ts.count++] = OptTensor{p[i], g[i], numel[i] | (uint64_t)p_dtype[i] << 48 | (uint64_t)g_dtype[i] << 52,
-                                             (uint32_t)(offset[i] / kOptBlock), (uint32_t)blocks};
+            a.p[k] = (uint64_t)(uintptr_t)p[i] | (uint64_t)p_dtype[i] << 48;
+            a.g[k] = g[i] ? (uint64_t)(uintptr_t)g[i] | (uint64_t)g_dtype[i] << 48 : 0;
+            any |= g[i] && c;
             blocks += c;
         }
-        a.ts.counter0 = (uint32_t)done;
+        a.chunk0 = (uint32_t)done;
         done += blocks;
         if (any) HIP_TRY(launch_adamw_many(a, mo->bits, (uint32_t)blocks, (hipStream_t)stream));
     }
@@ -144,10 +170,10 @@ int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, con
             const uint64_t c = g[i] ? chunks_of(numel[i], per) : 0;
             if (blocks + c > kMaxBlocks) break;
             if (!c) continue;
-            ts.t[ts.count++] = OptTensor{nullptr, g[i], numel[i] | (uint64_t)dtype[i] << 48, 0, (uint32_t)blocks};
+            ts.t[ts.count++] = list_entry(g[i], numel[i], dtype[i], blocks);
             blocks += c;
         }
-        ts.counter0 = (uint32_t)done;
+        ts.partial0 = (uint32_t)done;
         done += blocks;
         if (blocks) HIP_TRY(launch_norm_partial(ts, (uint32_t)blocks, per, (double*)scratch, (hipStream_t)stream));
     }
@@ -160,7 +186,7 @@ int srgen_scale_many(int count, void* const* g, const uint64_t* numel, const int
     if (int rc = check_list(count, g, numel, dtype, "tensor", true)) return rc;
     if (!coef) return fail(SRGEN_E_INVALID, "coef is NULL");
     OptTensors ts;
-    ts.counter0 = 0;
+    ts.partial0 = 0;
     for (int i = 0; i < count; ++i)
         if (numel[i] && !g[i]) return fail(SRGEN_E_INVALID, "tensor %d is NULL", i);
     for (int i = 0; i < count;) {
@@ -170,7 +196,7 @@ int srgen_scale_many(int count, void* const* g, const uint64_t* numel, const int
             const uint64_t c = chunks_of(numel[i], kOptChunk);
             if (blocks + c > kMaxBlocks) break;
             if (!c) continue;
-            ts.t[ts.count++] = OptTensor{g[i], nullptr, numel[i] | (uint64_t)dtype[i] << 48, 0, (uint32_t)blocks};
+            ts.t[ts.count++] = list_entry(g[i], numel[i], dtype[i], blocks);
             blocks += c;
         }
         if (blocks) HIP_TRY(launch_scale_many(ts, (uint32_t)blocks, coef, (hipStream_t)stream));

@@ -119,7 +119,11 @@ class Moments:
             self.root_scale = byte(self.total // BLOCK, 1).view(torch.float8_e8m0fnu)
             ptrs = tuple(t.data_ptr() for t in (self.exp_avg, self.root, self.exp_avg_scale, self.root_scale))
         self._numel, self._offset = array("Q", self.numels), array("Q", self.offsets)
-        self._c = _lib.srgen_moments(bits, 0, *ptrs, self.step.data_ptr(), self.total, self.counter0[-1])
+        chunks = self.counter0[-1]
+        table = torch.empty((chunks, 4), dtype=torch.int32)                    # which chunk is where: of the sizes alone
+        _lib.check(_lib.lib().srgen_adamw_chunk_table(len(self.numels), _addr(self._numel), _addr(self._offset), table.data_ptr(), chunks))
+        self._table = table.to(device)
+        self._c = _lib.srgen_moments(bits, 0, *ptrs, self.step.data_ptr(), self._table.data_ptr(), self.total, chunks)
 
     @property
     def nbytes(self) -> int:

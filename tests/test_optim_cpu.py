@@ -18,7 +18,7 @@ def _lib():
 def _adamw(numel=(64,), offset=(0,), p=(4096,), g=(8192,), pd=(0,), gd=(0,), count=None, **over):
     """srgen_adamw_many with addresses that are never followed: every call here is refused before anything is launched."""
     L = _lib()
-    mo = L.srgen_moments(32, 0, 1 << 20, 1 << 21, None, None, 1 << 22, 64, 1)
+    mo = L.srgen_moments(32, 0, 1 << 20, 1 << 21, None, None, 1 << 22, 1 << 23, 64, 1)
     args = L.srgen_adamw_args(1e-3, 0.9, 0.999, 1e-8, 0.0, None, None, None, None, 0, 0)
     for k, v in over.items():
         setattr(mo if hasattr(mo, k) else args, k, v)
@@ -40,7 +40,11 @@ def _adamw(numel=(64,), offset=(0,), p=(4096,), g=(8192,), pd=(0,), gd=(0,), cou
     (dict(offset=(16,)), -1, "offset"),
     (dict(offset=(32,)), -1, "end behind their buffer"),
     (dict(numel=(65,)), -1, "end behind their buffer"),
-    (dict(counters=0), -1, "step counters"),
+    (dict(chunks=0), -1, "chunks"),
+    (dict(chunks=2), -1, "chunks"),
+    (dict(p=(1 << 50,)), -6, "48 bits"),
+    (dict(table=None), -1, "NULL moments"),
+    (dict(table=(1 << 23) + 8), -1, "misaligned"),
     (dict(numel=(1 << 40,)), -6, "elements"),
     (dict(m=None), -1, "NULL moments"),
     (dict(step=None), -1, "NULL moments"),
@@ -59,8 +63,8 @@ def test_adamw_many_refuses(kw, rc, text):
 
 
 def test_empty_lists_are_allowed():
-    assert _adamw(numel=(), offset=(), p=(), g=(), pd=(), gd=())[0] == 0
-    assert _adamw(numel=(0, 0), offset=(0, 0), p=(0, 0), g=(0, 0), pd=(0, 0), gd=(0, 0))[0] == 0
+    assert _adamw(numel=(), offset=(), p=(), g=(), pd=(), gd=(), chunks=0)[0] == 0
+    assert _adamw(numel=(0, 0), offset=(0, 0), p=(0, 0), g=(0, 0), pd=(0, 0), gd=(0, 0), chunks=0)[0] == 0
     L = _lib().lib()
     z, d = array("Q", [0]), array("i", [0])
     assert L.srgen_scale_many(1, z.buffer_info()[0], z.buffer_info()[0], d.buffer_info()[0], 64, None) == 0
@@ -71,10 +75,16 @@ def test_counters_and_scratch():
     L = _lib().lib()
     n = array("Q", [0, 1, 4096, 4097])
     out = ctypes.c_uint64()
-    assert L.srgen_adamw_counters(4, n.buffer_info()[0], ctypes.byref(out)) == 0 and out.value == 0 + 1 + 1 + 2
+    assert L.srgen_adamw_chunk_count(4, n.buffer_info()[0], ctypes.byref(out)) == 0 and out.value == 0 + 1 + 1 + 2
+    off, table = array("Q", [0, 0, 32, 4128]), array("I", bytes(64))
+    assert L.srgen_adamw_chunk_table(4, n.buffer_info()[0], off.buffer_info()[0], table.buffer_info()[0], 4) == 0
+    assert list(table) == [1, 0, 0, 1, 2, 0, 1, 4096, 3, 0, 129, 4096, 3, 1, 257, 1]
+    assert L.srgen_adamw_chunk_table(4, n.buffer_info()[0], off.buffer_info()[0], table.buffer_info()[0], 3) == -1
+    off[1] = 16
+    assert L.srgen_adamw_chunk_table(4, n.buffer_info()[0], off.buffer_info()[0], table.buffer_info()[0], 4) == -1
     b = ctypes.c_size_t()
     assert L.srgen_total_norm_scratch_bytes(4, n.buffer_info()[0], ctypes.byref(b)) == 0 and b.value >= 4 * 8
-    assert L.srgen_adamw_counters(4, None, ctypes.byref(out)) == -1
+    assert L.srgen_adamw_chunk_count(4, None, ctypes.byref(out)) == -1
     assert L.srgen_total_norm_scratch_bytes(-1, n.buffer_info()[0], ctypes.byref(b)) == -1
 
 
