@@ -403,21 +403,71 @@ __device__ inline double wave_sum(double x)
     return x;
 }
 
+// 16 bytes of a list's tensor as 64-bit squares' sum; any alignment of the element
+template <int DT>
+struct Vec16 {
+    static constexpr int N = DT == 0 ? 4 : 8;
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef unsigned short h8 __attribute__((ext_vector_type(8), aligned(2)));
+    union {
+        f4 f;
+        h8 h;
+    };
+    __device__ inline void load(const void* p, uint64_t i)
+    {
+        if constexpr (DT == 0) f = *(const GLOBAL f4*)((const GLOBAL float*)p + i);
+        else h = *(const GLOBAL h8*)((const GLOBAL unsigned short*)p + i);
+    }
+    __device__ inline double add(double acc) const
+    {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const double x = DT == 0 ? (double)f[k] : DT == 1 ? (double)bf16_to_f32(h[k]) : (double)(float)__builtin_bit_cast(_Float16, (unsigned short)h[k]);
+            acc = fma(x, x, acc);
+        }
+        return acc;
+    }
+};
+
+template <int DT>
+__device__ inline double sum_squares(const void* p, uint64_t base, uint64_t end)
+{
+    constexpr int N = Vec16<DT>::N, U = 4;                 // four loads of 16 bytes requested before the first is used
+    constexpr uint32_t STEP = 256 * N;
+    double acc = 0.0;
+    uint64_t i = base + threadIdx.x * N;
+    for (; i + (U - 1) * STEP + N <= end; i += U * STEP) {
+        Vec16<DT> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u].load(p, i + u * STEP);
+#pragma unroll
+        for (int u = 0; u < U; ++u) acc = x[u].add(acc);
+    }
+    for (; i < end; i += STEP) {
+        if (i + N <= end) {
+            Vec16<DT> x;
+            x.load(p, i);
+            acc = x.add(acc);
+        } else {
+            for (uint64_t k = i; k < end; ++k) {
+                const double x = DT == 0 ? (double)((const GLOBAL float*)p)[k]
+                               : DT == 1 ? (double)bf16_to_f32(((const GLOBAL unsigned short*)p)[k])
+                                         : (double)(float)__builtin_bit_cast(_Float16, ((const GLOBAL unsigned short*)p)[k]);
+                acc = fma(x, x, acc);
+            }
+        }
+    }
+    return acc;
+}
+
 // sums of squares in 64 bits, in a fixed order: one partial sum for each workgroup's elements
 __global__ __launch_bounds__(256) void norm_partial_kernel(const OptTensors ts, uint32_t per_block, double* __restrict__ partial)
 {
     __shared__ double red[4];
     const Found f = find_tensor(ts, blockIdx.x);
-    const uint64_t n = f.n;
     const uint64_t base = (uint64_t)f.block * per_block;
-    const uint64_t end = base + per_block < n ? base + per_block : n;
-    double acc = 0.0;
-    for (uint64_t i = base + threadIdx.x * 4; i < end; i += 1024) {
-        float g[4];
-        load_quad_dt(f.dt, f.base, i, n, g);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc = fma((double)g[k], (double)g[k], acc);
-    }
+    const uint64_t end = base + per_block < f.n ? base + per_block : f.n;
+    double acc = f.dt == 0 ? sum_squares<0>(f.base, base, end) : f.dt == 1 ? sum_squares<1>(f.base, base, end) : sum_squares<2>(f.base, base, end);
     acc = wave_sum(acc);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
     __syncthreads();

@@ -24,6 +24,7 @@ from operator import attrgetter
 from typing import List, Optional, Tuple
 
 import torch
+from torch.optim import optimizer as _torch_optimizer
 
 from . import _lib
 
@@ -36,15 +37,16 @@ except ImportError as e:
 BLOCK = 32            # SRGEN_OPT_BLOCK: elements that share one scale (8-bit moments)
 CHUNK = 4096          # SRGEN_OPT_CHUNK: elements of one step counter
 
+_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(dev).cuda_stream without the object
 _CODE = {torch.float32: _lib.SRGEN_F32, torch.bfloat16: _lib.SRGEN_BF16, torch.float16: _lib.SRGEN_F16}
 _TYPES = frozenset((torch.float32, torch.bfloat16))                  # of parameters and their gradients
-_dtype_of = attrgetter("dtype")
+_dtype_of, _device_of = attrgetter("dtype"), attrgetter("device")
 _data_ptr = torch.Tensor.data_ptr
 _numel = torch.Tensor.numel
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return _raw_stream(dev.index)
 
 
 def _on(dev: torch.device):
@@ -73,7 +75,7 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _one_device(tensors, what: str) -> torch.device:
-    devs = {t.device for t in tensors}
+    devs = set(map(_device_of, tensors))
     if len(devs) != 1 or next(iter(devs)).type != "cuda":
         raise RuntimeError(f"{what}: tensors of one ROCm device, got {sorted(map(str, devs))}; there is no CPU fallback")
     return next(iter(devs))
@@ -119,6 +121,7 @@ class Moments:
             self.root_scale = byte(self.total // BLOCK, 1).view(torch.float8_e8m0fnu)
             ptrs = tuple(t.data_ptr() for t in (self.exp_avg, self.root, self.exp_avg_scale, self.root_scale))
         self._numel, self._offset = array("Q", self.numels), array("Q", self.offsets)
+        self._sizes = _addr(self._numel), _addr(self._offset)
         chunks = self.counter0[-1]
         table = torch.empty((chunks, 4), dtype=torch.int32)                    # which chunk is where: of the sizes alone
         _lib.check(_lib.lib().srgen_adamw_chunk_table(len(self.numels), _addr(self._numel), _addr(self._offset), table.data_ptr(), chunks))
@@ -157,8 +160,12 @@ class Moments:
 
     def update(self, p: array, g: array, p_dtype: array, g_dtype: array, args: "_lib.srgen_adamw_args", stream: int) -> None:
         """One AdamW step of the list (addresses and type codes in the list's order; address 0: no gradient)."""
-        _lib.check(_lib.lib().srgen_adamw_many(len(self.numels), _addr(p), _addr(g), _addr(self._numel), _addr(self._offset),
-                                               _addr(p_dtype), _addr(g_dtype), self._c, args, stream))
+        self._update((_addr(p), _addr(g)), (_addr(p_dtype), _addr(g_dtype)), args, stream)
+
+    def _update(self, pg, codes, args, stream: int) -> None:
+        rc = _lib.lib().srgen_adamw_many(len(self.numels), *pg, *self._sizes, *codes, self._c, args, stream)
+        if rc:
+            _lib.check(rc)
 
 
 def _pack_into(exp_avg, exp_avg_sq, m8, me, r8, re) -> None:
@@ -176,8 +183,8 @@ def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor):
         if t.dtype != torch.float32 or t.dim() != 1 or not t.is_contiguous() or t.shape != exp_avg.shape:
             raise RuntimeError(f"pack_moments: two flat contiguous fp32 tensors of one length, got {tuple(t.shape)} {t.dtype}")
     n = _up(exp_avg.numel(), BLOCK)
-    m8, r8 = (torch.empty(n, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
-    me, re = (torch.empty(n // BLOCK, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu) for _ in range(2))
+    m8, r8 = (torch.empty(n, dtype=torch.float8_e4m3fn, device=dev) for _ in range(2))
+    me, re = (torch.empty(n // BLOCK, dtype=torch.float8_e8m0fnu, device=dev) for _ in range(2))
     _pack_into(exp_avg, exp_avg_sq, m8, me, r8, re)
     return m8, me, r8, re
 
@@ -230,7 +237,7 @@ def _listed(tensors: List[torch.Tensor], what: str):
             if t.layout != torch.strided:
                 raise RuntimeError(f"{what}: strided tensors, got {t.layout}")
         code = _codes(tensors, what)
-        tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
+        tensors = [t if t.is_contiguous() or _dense(t) else t.detach().contiguous() for t in tensors]
         ptr, numel = array("Q", map(_data_ptr, tensors)), array("Q", map(_numel, tensors))
     return dev, tensors, ptr, numel, code
 
@@ -247,10 +254,9 @@ def _norm_coef(dev: torch.device, ptr: array, numel: array, code: array, max_nor
     return buf[words:]
 
 
-@torch.no_grad()
 def total_norm(tensors) -> torch.Tensor:
     """The L2 norm of all ``tensors`` (fp32, bf16, fp16) taken together, as a 0-dim fp32 device tensor
-    (``torch.nn.utils.get_total_norm``).  Sums are held in 64 bits and added in a fixed order: the result does not overflow
+    (``torch.nn.utils.get_total_norm``; not differentiable).  Sums are held in 64 bits and added in a fixed order: the result does not overflow
     before the norm itself does, and repeats bit for bit."""
     ts = _tensor_list(tensors)
     if not ts:
@@ -296,12 +302,16 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
 
 
 # ---- AdamW -------------------------------------------------------------------------------------------------------------
+_GLOBAL_HOOKS = (_torch_optimizer._global_optimizer_pre_hooks, _torch_optimizer._global_optimizer_post_hooks)
+
+
 class _Lists:
     """A group's addresses and type codes, as the kernels' list wants them; filled anew at every step."""
 
     def __init__(self, n: int):
         self.p, self.g, self.p_code = _arrays(n)
         self.g_code = array("i", self.p_code)
+        self.pg, self.codes = (_addr(self.p), _addr(self.g)), (_addr(self.p_code), _addr(self.g_code))
         self.checked = (array("Q"), array("i"))            # parameters' addresses and types that were last found apart
 
 
@@ -370,8 +380,17 @@ class AdamW(torch.optim.Optimizer):
         self._lists.append(_Lists(len(g["params"])))
 
     # -- one step -----------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None):
+        # torch wraps the step() of every optimizer in a profiler range and its hooks, which takes longer than a small step does:
+        # here only where a profiler runs or somebody has registered a hook
+        if (torch._C._autograd._profiler_enabled() or self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks
+                or any(_GLOBAL_HOOKS)):
+            return self._step_with_hooks(closure)
+        return self._step(closure)
+
+    step.hooked = True                                     # (how torch's wrapper marks the ones it has wrapped)
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -422,12 +441,15 @@ class AdamW(torch.optim.Optimizer):
                 args = _lib.srgen_adamw_args(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev,
                                              None if norm_coef is None else norm_coef.data_ptr() + 4, None if div is None else div.data_ptr(),
                                              None if found is None else found.data_ptr(), self.seed, 1 if group["maximize"] else 0)
-                mo.update(ls.p, ls.g, ls.p_code, ls.g_code, args, stream)
+                mo._update(ls.pg, ls.codes, args, stream)
                 # the kernel wrote behind torch's back: the version counters are what the Generator / Discriminator mirrors
                 # watch to upload their weights again
                 _tensorlist.bump(group["params"], ls.g)
         return loss
 
+    _step_with_hooks = torch.optim.Optimizer.profile_hook_step(_step)
+
+    @torch.no_grad()
     def _look_closer(self, k: int, kept: list) -> int:
         """Group ``k`` has a tensor that is not plain (contiguous fp32 or bf16, on the device, of the size it was added with):
         refused, or its gradient brought into the parameter's order; such copies are put into ``kept``."""
