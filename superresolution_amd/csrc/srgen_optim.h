@@ -65,8 +65,8 @@ static_assert(sizeof(OptTensors) <= 4096 - 64, "kernel arguments hold 4 KiB");
 
 uint32_t opt_mix(uint32_t x);        // the hash of the stochastic rounding (host side, for the seed)
 
-hipError_t launch_adamw_many(const AdamWArgs& a, int bits, uint32_t blocks, hipStream_t s);
-hipError_t launch_norm_partial(const OptTensors& ts, uint32_t blocks, uint32_t per_block, double* partial, hipStream_t s);
+hipError_t launch_adamw_many(const AdamWArgs& a, int bits, bool streaming, uint32_t blocks, hipStream_t s);
+hipError_t launch_norm_partial(const OptTensors& ts, bool streaming, uint32_t blocks, uint32_t per_block, double* partial, hipStream_t s);
 hipError_t launch_norm_final(const double* partial, uint32_t n, double max_norm, float* norm_coef, hipStream_t s);
 hipError_t launch_scale_many(const OptTensors& ts, uint32_t blocks, const float* coef, hipStream_t s);
 hipError_t launch_moments_pack(const float* m, const float* v, size_t n, uint8_t* m8, uint8_t* me, uint8_t* r8, uint8_t* re,

@@ -24,6 +24,10 @@ namespace {
 // workgroups of 256 threads in one launch: the grid is counted in threads, in 32 bits
 constexpr uint64_t kMaxBlocks = (1ull << 24) - 1;
 
+// A step that moves more than this past the 256 MB Infinity Cache finds nothing of it there at the next step: its loads and stores
+// are marked non-temporal.
+constexpr uint64_t kStreamingBytes = 256ull << 20;
+
 inline size_t element_bytes(int dtype) { return dtype == SRGEN_F32 ? 4 : 2; }
 inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 inline uint64_t chunks_of(uint64_t n, uint64_t per) { return (n + per - 1) / per; }
@@ -100,8 +104,9 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
     if (!(args->lr >= 0.0) || !(args->eps >= 0.0) || !(args->weight_decay >= 0.0) || !(args->beta1 >= 0.0 && args->beta1 < 1.0) ||
         !(args->beta2 >= 0.0 && args->beta2 < 1.0))
         return fail(SRGEN_E_INVALID, "lr %g, betas %g %g, eps %g, weight decay %g", args->lr, args->beta1, args->beta2, args->eps, args->weight_decay);
-    uint64_t chunks = 0;
+    uint64_t chunks = 0, step_bytes = 0;
     for (int i = 0; i < count; ++i) {
+        if (g[i]) step_bytes += numel[i] * (2 * element_bytes(p_dtype[i]) + element_bytes(g_dtype[i]) + (mo->bits == 32 ? 16 : 4));
         if (numel[i] && !p[i]) return fail(SRGEN_E_INVALID, "parameter %d is NULL", i);
         if (offset[i] % kOptBlock || offset[i] / kOptBlock > 0xFFFFFFFFull) return fail(SRGEN_E_INVALID, "offset %d: %llu", i, (unsigned long long)offset[i]);
         if (offset[i] + chunks_of(numel[i], kOptBlock) * kOptBlock > mo->numel)
@@ -118,6 +123,7 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
     a.sc = AdamWScalars{args->beta1, args->beta2, log(args->beta1), log(args->beta2), args->lr, args->eps, args->weight_decay,
                         args->lr_dev, args->grad_mul, args->grad_div, args->found_inf, opt_mix(args->seed), args->maximize};
     a.mo = MomentPtrs{mo->m, mo->v, mo->m_scale, mo->v_scale, mo->step, reinterpret_cast<const OptChunk*>(mo->table)};
+    const bool streaming = step_bytes > kStreamingBytes;
     uint64_t done = 0;                                     // chunks of the launches so far
     for (int i = 0; i < count;) {
         uint64_t blocks = 0;
@@ -134,7 +140,7 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
         }
         a.chunk0 = (uint32_t)done;
         done += blocks;
-        if (any) HIP_TRY(launch_adamw_many(a, mo->bits, (uint32_t)blocks, (hipStream_t)stream));
+        if (any) HIP_TRY(launch_adamw_many(a, mo->bits, streaming, (uint32_t)blocks, (hipStream_t)stream));
     }
     return SRGEN_OK;
 }
@@ -155,8 +161,12 @@ int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, con
     if (int rc = check_list(count, g, numel, dtype, "tensor", true)) return rc;
     if (!norm_coef2) return fail(SRGEN_E_INVALID, "norm_coef2 is NULL");
     const uint32_t per = norm_per_block(count, numel);
-    uint64_t total = 0;
-    for (int i = 0; i < count; ++i) total += g[i] ? chunks_of(numel[i], per) : 0;
+    uint64_t total = 0, bytes = 0;
+    for (int i = 0; i < count; ++i) {
+        if (!g[i]) continue;
+        total += chunks_of(numel[i], per);
+        bytes += numel[i] * element_bytes(dtype[i]);
+    }
     if (total > 0xFFFFFFFFull) return fail(SRGEN_E_UNSUPPORTED, "%llu partial sums", (unsigned long long)total);
     if (total && (!scratch || !aligned(scratch, 8))) return fail(SRGEN_E_INVALID, "scratch is NULL or misaligned");
     if (scratch_bytes < total * sizeof(double))
@@ -175,7 +185,7 @@ int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, con
         }
         ts.partial0 = (uint32_t)done;
         done += blocks;
-        if (blocks) HIP_TRY(launch_norm_partial(ts, (uint32_t)blocks, per, (double*)scratch, (hipStream_t)stream));
+        if (blocks) HIP_TRY(launch_norm_partial(ts, bytes > kStreamingBytes, (uint32_t)blocks, per, (double*)scratch, (hipStream_t)stream));
     }
     HIP_TRY(launch_norm_final((const double*)scratch, (uint32_t)total, max_norm, norm_coef2, (hipStream_t)stream));
     return SRGEN_OK;

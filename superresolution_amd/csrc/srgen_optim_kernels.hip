@@ -7,7 +7,9 @@ namespace {
 
 // unaligned vectors: a gradient that is a view into a flat buffer starts at any element (global loads need element alignment only)
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 // an address that came as a number is in device memory: without this it would be reached by flat loads
 #define GLOBAL __attribute__((address_space(1)))
 
@@ -26,46 +28,78 @@ __device__ inline float bf16_to_f32(uint32_t h) { return __uint_as_float(h << 16
 
 __device__ inline uint32_t round_up_block(uint32_t n) { return (n + kOptBlock - 1) & ~(uint32_t)(kOptBlock - 1); }
 
-// four consecutive elements from `i` of `n`; behind the end: zeros.  DT: 0 fp32, 1 bf16, 2 fp16
+template <bool NT, typename T>
+__device__ inline T load_as(const GLOBAL T* p)
+{
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool NT, typename T>
+__device__ inline void store_as(T x, GLOBAL T* p)
+{
+    if constexpr (NT) __builtin_nontemporal_store(x, p);
+    else *p = x;
+}
+
+// Four consecutive elements as they are in memory (values() converts: a conversion beside the load would wait for it).
+// DT: 0 fp32, 1 bf16, 2 fp16.
 template <int DT>
 struct Quad {
-    static __device__ inline void load(const void* base, uint64_t i, uint64_t n, float (&x)[4])
+    u16x4 h;
+    __device__ inline void values(float (&x)[4]) const
     {
-        if constexpr (DT == 0) {
-            const GLOBAL float* q = (const GLOBAL float*)base + i;
-            f32x4u a = {0.f, 0.f, 0.f, 0.f};
-            if (i + 4 <= n) a = *(const GLOBAL f32x4u*)q;
-            else if (i < n) {
-                a[0] = q[0];
-                if (i + 1 < n) a[1] = q[1];
-                if (i + 2 < n) a[2] = q[2];
-            }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = a[k];
-        } else {
-            const GLOBAL unsigned short* q = (const GLOBAL unsigned short*)base + i;
-            u16x4u a = {0, 0, 0, 0};
-            if (i + 4 <= n) a = *(const GLOBAL u16x4u*)q;
-            else if (i < n) {
-                a[0] = q[0];
-                if (i + 1 < n) a[1] = q[1];
-                if (i + 2 < n) a[2] = q[2];
-            }
+        for (int k = 0; k < 4; ++k)
+            x[k] = DT == 1 ? bf16_to_f32(h[k]) : (float)__builtin_bit_cast(_Float16, (unsigned short)h[k]);
+    }
+};
+template <>
+struct Quad<0> {
+    f32x4 f;
+    __device__ inline void values(float (&x)[4]) const
+    {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                x[k] = DT == 1 ? bf16_to_f32(a[k]) : (float)__builtin_bit_cast(_Float16, (unsigned short)a[k]);
-        }
+        for (int k = 0; k < 4; ++k) x[k] = f[k];
     }
 };
 
-__device__ inline void store_f32(void* base, uint64_t i, uint64_t n, const float (&x)[4])
+// elements i .. i + 3 of `n`; behind the end: zeros.  FULL: all four are there.  The index counts from a base that is the same
+// for the workgroup, in 32 bits.
+template <int DT, bool FULL, bool NT>
+__device__ inline Quad<DT> load_quad(const void* base, uint32_t i, uint32_t n)
+{
+    Quad<DT> a;
+    if constexpr (DT == 0) {
+        const GLOBAL float* q = (const GLOBAL float*)base + i;
+        if (!FULL) a.f = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (FULL || i + 4 <= n) a.f = load_as<NT>((const GLOBAL f32x4u*)q);
+        else if (i < n) {
+            a.f[0] = q[0];
+            if (i + 1 < n) a.f[1] = q[1];
+            if (i + 2 < n) a.f[2] = q[2];
+        }
+    } else {
+        const GLOBAL unsigned short* q = (const GLOBAL unsigned short*)base + i;
+        if (!FULL) a.h = u16x4{0, 0, 0, 0};
+        if (FULL || i + 4 <= n) a.h = load_as<NT>((const GLOBAL u16x4u*)q);
+        else if (i < n) {
+            a.h[0] = q[0];
+            if (i + 1 < n) a.h[1] = q[1];
+            if (i + 2 < n) a.h[2] = q[2];
+        }
+    }
+    return a;
+}
+
+template <bool FULL, bool NT>
+__device__ inline void store_f32(void* base, uint32_t i, uint32_t n, const float (&x)[4])
 {
     GLOBAL float* q = (GLOBAL float*)base + i;
-    if (i + 4 <= n) {
+    if (FULL || i + 4 <= n) {
         f32x4u a;
 #pragma unroll
         for (int k = 0; k < 4; ++k) a[k] = x[k];
-        *(GLOBAL f32x4u*)q = a;
+        store_as<NT>(a, (GLOBAL f32x4u*)q);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -73,14 +107,15 @@ __device__ inline void store_f32(void* base, uint64_t i, uint64_t n, const float
     }
 }
 
-__device__ inline void store_u16(void* base, uint64_t i, uint64_t n, const unsigned short (&x)[4])
+template <bool FULL, bool NT>
+__device__ inline void store_u16(void* base, uint32_t i, uint32_t n, const unsigned short (&x)[4])
 {
     GLOBAL unsigned short* q = (GLOBAL unsigned short*)base + i;
-    if (i + 4 <= n) {
+    if (FULL || i + 4 <= n) {
         u16x4u a;
 #pragma unroll
         for (int k = 0; k < 4; ++k) a[k] = x[k];
-        *(GLOBAL u16x4u*)q = a;
+        store_as<NT>(a, (GLOBAL u16x4u*)q);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -119,7 +154,7 @@ __device__ inline uint32_t finite_bits(float x)
 template <int CTRL>
 __device__ inline uint32_t max_dpp(uint32_t x)
 {
-    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xF, 0xF, false);
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);   // (0: one instruction with the max)
     return x > o ? x : o;
 }
 __device__ inline uint32_t max8(uint32_t x)                  // over the 8 lanes that hold one block: neighbours, pairs, the two quads
@@ -127,12 +162,18 @@ __device__ inline uint32_t max8(uint32_t x)                  // over the 8 lanes
     return max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(x)));  // quad_perm [1,0,3,2], quad_perm [2,3,0,1], row_half_mirror
 }
 
-// the scale byte of a block whose lane holds x[0..3]; magnitudes above kTop are brought down to it (a branch that is hardly
-// ever taken: the maximum shows whether there is one, v_max skips NaN)
+// The scale byte of a block whose lane holds x[0..3]; magnitudes above kTop are brought down to it, in a branch that is hardly
+// ever taken (v_max skips NaN; in a root's bits NaN is above everything).  ROOT: no x is negative.
+template <bool ROOT>
 __device__ inline uint32_t block_scale(float (&x)[4])
 {
-    float t = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-    uint32_t top = max8(__float_as_uint(t) & 0x7FFFFFFFu);
+    uint32_t t;
+    if constexpr (ROOT) {
+        const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]), c = __float_as_uint(x[2]), d = __float_as_uint(x[3]);
+        const uint32_t ab = a > b ? a : b, cd = c > d ? c : d;
+        t = ab > cd ? ab : cd;
+    } else t = __float_as_uint(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+    uint32_t top = max8(t);
     if (__builtin_expect(top > kTop, 0)) {                   // (the same in all 8 lanes)
         uint32_t b = 0;
 #pragma unroll
@@ -146,25 +187,34 @@ __device__ inline uint32_t block_scale(float (&x)[4])
     return scale_byte(top);
 }
 
-// four codes; ROOT: what is not zero is raised to the smallest code, 2^-9 of the scale (med3 of x, that, and x times a power
-// of two no root is too small for: a root is 0 or at least 2^-75)
-template <bool ROOT>
+// four codes
 __device__ inline uint32_t e4m3_codes(const float (&x)[4], uint32_t e, const uint32_t (&seed)[4])
 {
     const float s = __uint_as_float(e << 23);
     int c = 0;
-    float y[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] = ROOT ? __builtin_amdgcn_fmed3f(x[k], s * 0x1p-9f, x[k] * 0x1p126f) : x[k];
-    if (ROOT && __builtin_expect(__builtin_isunordered(x[0], x[1]) || __builtin_isunordered(x[2], x[3]), 0)) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = x[k] != x[k] ? x[k] : y[k];           // (med3 passes over NaN)
-    }
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, y[0], seed[0], s, 0);
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, y[1], seed[1], s, 1);
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, y[2], seed[2], s, 2);
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, y[3], seed[3], s, 3);
+    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[0], seed[0], s, 0);
+    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[1], seed[1], s, 1);
+    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[2], seed[2], s, 2);
+    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[3], seed[3], s, 3);
     return (uint32_t)c;
+}
+
+// the same for roots: what is not zero is raised to the smallest code, 2^-9 of the scale.  `plain`: none is 0 or NaN (roots())
+__device__ inline uint32_t e4m3_root_codes(const float (&x)[4], bool plain, uint32_t e, const uint32_t (&seed)[4])
+{
+    const float q = __uint_as_float(e << 23) * 0x1p-9f;
+    float y[4];
+    if (__builtin_expect(plain, 1)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                        // (as whole numbers: the same order, and no care for NaN)
+            const uint32_t a = __float_as_uint(x[k]), b = __float_as_uint(q);
+            y[k] = __uint_as_float(a > b ? a : b);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = x[k] > 0.f && x[k] < q ? q : x[k];
+    }
+    return e4m3_codes(y, e, seed);
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -178,12 +228,14 @@ __device__ inline void e4m3_values(uint32_t c, uint32_t e, float (&x)[4])
     x[3] = b[1];
 }
 
-// square roots to the nearest: y ~ 1 / sqrt(v), s = v y, then the residual v - s^2, exact in one fma, put right with y / 2.  That
-// is within 2^-45 of the root before the last rounding; below 2^-90 (the residual would underflow), at 0 and at infinity sqrtf
-__device__ inline void roots(const float (&v)[4], float (&r)[4])
+// Square roots to the nearest: y ~ 1 / sqrt(v), s = v y, then the residual v - s^2, exact in one fma, put right with y / 2.
+// That is within 2^-45 of the root before the last rounding.  Below 2^-90 (the residual would underflow), at 0, infinity and NaN
+// sqrtf instead; returns whether there was none of these.
+__device__ inline bool roots(const float (&v)[4], float (&r)[4])
 {
     const float lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), hi = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-    if (__builtin_expect(lo >= 0x1p-90f && hi < INFINITY, 1)) {
+    const bool plain = lo >= 0x1p-90f && hi < INFINITY && !__builtin_isunordered(v[0], v[1]) && !__builtin_isunordered(v[2], v[3]);
+    if (__builtin_expect(plain, 1)) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float y = __builtin_amdgcn_rsqf(v[k]);
@@ -194,6 +246,7 @@ __device__ inline void roots(const float (&v)[4], float (&r)[4])
 #pragma unroll
         for (int k = 0; k < 4; ++k) r[k] = sqrtf(v[k]);
     }
+    return plain;
 }
 
 // ---- AdamW -------------------------------------------------------------------------------------------------------------
@@ -209,163 +262,190 @@ struct StepScalars {
 };
 
 // what a thread reads for its four elements
-template <int BITS>
+template <int BITS, int PDT, int GDT>
 struct Operands {
-    float p[4], g[4];
-    float4 m, v;                       // 32 bits
+    Quad<PDT> p;
+    Quad<GDT> g;
+    f32x4 m, v;                        // 32 bits
     uint32_t mc, vc, me, ve;           // 8 bits
 };
 
-template <int BITS, int PDT, int GDT>
-__device__ inline void load_operands(const AdamWArgs& a, const OptChunk& ck, const void* pp, const void* gp, uint32_t i, Operands<BITS>& d)
+// a chunk's operands: bases are the same for the workgroup, indexes count from them
+struct Chunk {
+    void* p;
+    const void* g;
+    uint8_t* m;                        // (bytes)
+    uint8_t* v;
+    uint8_t* me;
+    uint8_t* ve;
+    uint32_t n, np;                    // elements; the same in whole blocks of 32 (8 lanes)
+    uint32_t lo, w;                    // position: its low word; that with the high word mixed in
+};
+
+template <int BITS, int PDT, int GDT, bool FULL, bool NT>
+__device__ inline void load_operands(const Chunk& c, uint32_t i, Operands<BITS, PDT, GDT>& d)
 {
-    const uint64_t off = (uint64_t)ck.offset32 * kOptBlock;
-    Quad<PDT>::load(pp, i, ck.count, d.p);
-    Quad<GDT>::load(gp, i, ck.count, d.g);
-    const bool in = i < round_up_block(ck.count);
+    d.p = load_quad<PDT, FULL, NT>(c.p, i, c.n);
+    d.g = load_quad<GDT, FULL, NT>(c.g, i, c.n);
     if constexpr (BITS == 32) {
-        d.m = d.v = float4{0.f, 0.f, 0.f, 0.f};
-        if (in) {
-            d.m = *(const float4*)((const float*)a.mo.m + off + i);
-            d.v = *(const float4*)((const float*)a.mo.v + off + i);
+        if (!FULL) d.m = d.v = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (FULL || i < c.np) {
+            d.m = load_as<NT>((const GLOBAL f32x4*)(c.m + i * 4));
+            d.v = load_as<NT>((const GLOBAL f32x4*)(c.v + i * 4));
         }
     } else {
-        d.mc = d.vc = d.me = d.ve = 0;
-        if (in) {
-            d.mc = *(const uint32_t*)((const uint8_t*)a.mo.m + off + i);
-            d.vc = *(const uint32_t*)((const uint8_t*)a.mo.v + off + i);
-            d.me = a.mo.m_scale[ck.offset32 + i / kOptBlock];
-            d.ve = a.mo.v_scale[ck.offset32 + i / kOptBlock];
+        if (!FULL) d.mc = d.vc = d.me = d.ve = 0;
+        if (FULL || i < c.np) {
+            d.mc = load_as<NT>((const GLOBAL uint32_t*)(c.m + i));
+            d.vc = load_as<NT>((const GLOBAL uint32_t*)(c.v + i));
+            d.me = ((const GLOBAL uint8_t*)c.me)[i / kOptBlock];
+            d.ve = ((const GLOBAL uint8_t*)c.ve)[i / kOptBlock];
         }
     }
 }
 
-template <int BITS, int PDT, int GDT>
-__device__ inline void adamw_chunk(const AdamWArgs& a, const OptChunk ck, void* pp, const void* gp, StepScalars* sh)
+template <int BITS, int PDT, int GDT, bool FULL, bool NT>
+__device__ inline void update(const AdamWScalars& sc, const StepScalars& sh, const Chunk& c, uint32_t i, Operands<BITS, PDT, GDT>& d)
+{
+    float m[4], r[4], p[4], g[4];
+    uint32_t h[4];
+    bool plain = true;
+    d.g.values(g);
+    d.p.values(p);
+    if (BITS == 8 || PDT == 1) {
+        uint32_t w = c.w + i;
+        if (!FULL && c.lo + i < c.lo) w += kGold;                      // (the high word goes up inside the chunk)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = mix32((w + k) ^ sh.key);
+    }
+    if constexpr (BITS == 32) {
+        const float b1 = (float)sc.beta1, d1 = (float)(1.0 - sc.beta1), b2 = (float)sc.beta2, d2 = (float)(1.0 - sc.beta2);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float gk = g[k] * sh.gmul;
+            d.m[k] = fmaf(b1, d.m[k], d1 * gk);
+            d.v[k] = fmaf(b2, d.v[k], (d2 * gk) * gk);
+            m[k] = d.m[k];
+            r[k] = sqrtf(d.v[k]);
+        }
+        store_as<NT>(d.m, (GLOBAL f32x4*)(c.m + i * 4));
+        store_as<NT>(d.v, (GLOBAL f32x4*)(c.v + i * 4));
+    } else {
+        float mo[4], ro[4], v[4];
+        e4m3_values(d.mc, d.me, mo);
+        e4m3_values(d.vc, d.ve, ro);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double gk = (double)g[k], rk = (double)ro[k];
+            m[k] = (float)fma(sc.beta1, (double)mo[k], sh.c1 * gk);
+            v[k] = (float)fma(sc.beta2, rk * rk, sh.c2 * (gk * gk));
+        }
+        plain = roots(v, r);
+    }
+    float x[4];
+    const float step = -sh.step, eps = (float)sc.eps;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = fmaf(step, m[k] * __builtin_amdgcn_rcpf(fmaf(r[k], sh.isb2, eps)), p[k] * sh.decay);
+    if constexpr (PDT == 0) store_f32<FULL, NT>(c.p, i, c.n, x);
+    else {
+        // bf16 by stochastic rounding: 16 random bits under the last kept one, the rest cut off.  (A NaN whose low bits the sum
+        // would carry out of is replaced by the plain one.)
+        unsigned short q[4];
+        if (__builtin_expect(__builtin_isunordered(x[0], x[1]) || __builtin_isunordered(x[2], x[3]), 0)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = x[k] != x[k] ? __uint_as_float(0x7FC00000u) : x[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = (unsigned short)((__float_as_uint(x[k]) + (mix32(h[k] + kGold) >> 16)) >> 16);
+        store_u16<FULL, NT>(c.p, i, c.n, q);
+    }
+    if constexpr (BITS == 8) {
+        uint32_t seed_m[4], seed_r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            seed_m[k] = h[k] << 16;
+            seed_r[k] = h[k] & 0xFFFF0000u;
+        }
+        const uint32_t em = block_scale<false>(m), er = block_scale<true>(r);
+        store_as<NT>(e4m3_codes(m, em, seed_m), (GLOBAL uint32_t*)(c.m + i));
+        store_as<NT>(e4m3_root_codes(r, plain, er, seed_r), (GLOBAL uint32_t*)(c.v + i));
+        if ((threadIdx.x & 7) == 0) {
+            ((GLOBAL uint8_t*)c.me)[i / kOptBlock] = (uint8_t)em;
+            ((GLOBAL uint8_t*)c.ve)[i / kOptBlock] = (uint8_t)er;
+        }
+    }
+}
+
+template <int BITS, int PDT, int GDT, bool FULL, bool NT>
+__device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScalars* shared)
 {
     const AdamWScalars& sc = a.sc;
-    const uint32_t n = ck.count, np = round_up_block(n);
-    const uint64_t off = (uint64_t)ck.offset32 * kOptBlock;
     const uint32_t tid = threadIdx.x;
-    Operands<BITS> d, next;
-    load_operands<BITS, PDT, GDT>(a, ck, pp, gp, tid * 4, d);
+    Operands<BITS, PDT, GDT> d, next;
+    load_operands<BITS, PDT, GDT, FULL, NT>(c, tid * 4, d);
     if (tid < 64) {
         int32_t* counter = a.mo.step + (size_t)a.chunk0 + blockIdx.x;
         const int t = *counter + 1;                                    // (this wave alone reads and writes it)
         const double lr = sc.lr_dev ? (double)*sc.lr_dev : sc.lr;
         const double bc1 = -expm1((double)t * sc.ln_beta1), bc2 = -expm1((double)t * sc.ln_beta2);
-        double c = sc.grad_mul ? (double)*sc.grad_mul : 1.0;
-        if (sc.grad_div) c /= (double)*sc.grad_div;
-        if (sc.negate) c = -c;
+        double f = sc.grad_mul ? (double)*sc.grad_mul : 1.0;
+        if (sc.grad_div) f /= (double)*sc.grad_div;
+        if (sc.negate) f = -f;
         if (tid == 0) {
             *counter = t;
-            sh->c1 = (1.0 - sc.beta1) * c;
-            sh->c2 = (1.0 - sc.beta2) * (c * c);
-            sh->decay = (float)(1.0 - lr * sc.wd);
-            sh->step = (float)(lr / bc1);
-            sh->isb2 = (float)(1.0 / sqrt(bc2));
-            sh->gmul = (float)c;
-            sh->key = mix32(sc.seed_key + (uint32_t)t * kGold);
+            shared->c1 = (1.0 - sc.beta1) * f;
+            shared->c2 = (1.0 - sc.beta2) * (f * f);
+            shared->decay = (float)(1.0 - lr * sc.wd);
+            shared->step = (float)(lr / bc1);
+            shared->isb2 = (float)(1.0 / sqrt(bc2));
+            shared->gmul = (float)f;
+            shared->key = mix32(sc.seed_key + (uint32_t)t * kGold);
         }
     }
     __syncthreads();
-    const float decay = sh->decay, step = -sh->step, isb2 = sh->isb2, eps = (float)sc.eps, gmul = sh->gmul;
-    const uint32_t key = sh->key;
-    const double c1 = sh->c1, c2 = sh->c2;
-
+    const StepScalars sh = *shared;
+    if constexpr (FULL) {
 #pragma unroll 2
-    for (uint32_t i0 = 0; i0 < kOptChunk; i0 += 1024) {
-        const uint32_t i = i0 + tid * 4;
-        if (i >= np) break;                                            // (whole blocks of 32: 8 lanes)
-        load_operands<BITS, PDT, GDT>(a, ck, pp, gp, i0 + 1024 < kOptChunk ? i + 1024 : kOptChunk, next);
-        const uint64_t j = off + i;
-        float m[4], r[4];
-        uint32_t h[4];
-        if (BITS == 8 || PDT == 1) {
-            const uint32_t w = (uint32_t)j + (uint32_t)(j >> 32) * kGold;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = mix32((w + k) ^ key);
+        for (uint32_t i0 = 0; i0 < kOptChunk; i0 += 1024) {
+            if (i0 + 1024 < kOptChunk) load_operands<BITS, PDT, GDT, FULL, NT>(c, i0 + 1024 + tid * 4, next);
+            update<BITS, PDT, GDT, FULL, NT>(sc, sh, c, i0 + tid * 4, d);
+            d = next;
         }
-        if constexpr (BITS == 32) {
-            const float b1 = (float)sc.beta1, d1 = (float)(1.0 - sc.beta1), b2 = (float)sc.beta2, d2 = (float)(1.0 - sc.beta2);
-            float* mq = (float*)&d.m;
-            float* vq = (float*)&d.v;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float gk = d.g[k] * gmul;
-                mq[k] = fmaf(b1, mq[k], d1 * gk);
-                vq[k] = fmaf(b2, vq[k], (d2 * gk) * gk);
-                m[k] = mq[k];
-                r[k] = sqrtf(vq[k]);
-            }
-            *(float4*)((float*)a.mo.m + j) = d.m;
-            *(float4*)((float*)a.mo.v + j) = d.v;
-        } else {
-            float mo[4], ro[4], v[4];
-            e4m3_values(d.mc, d.me, mo);
-            e4m3_values(d.vc, d.ve, ro);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const double gk = (double)d.g[k], rk = (double)ro[k];
-                m[k] = (float)fma(sc.beta1, (double)mo[k], c1 * gk);
-                v[k] = (float)fma(sc.beta2, rk * rk, c2 * (gk * gk));
-            }
-            roots(v, r);
-            float ms[4], rs[4];
-            uint32_t seed_m[4], seed_r[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                ms[k] = m[k];
-                rs[k] = r[k];
-                seed_m[k] = h[k] << 16;
-                seed_r[k] = h[k] & 0xFFFF0000u;
-            }
-            const uint32_t em = block_scale(ms), er = block_scale(rs);
-            *(uint32_t*)((uint8_t*)a.mo.m + j) = e4m3_codes<false>(ms, em, seed_m);
-            *(uint32_t*)((uint8_t*)a.mo.v + j) = e4m3_codes<true>(rs, er, seed_r);
-            if ((tid & 7) == 0) {
-                a.mo.m_scale[j / kOptBlock] = (uint8_t)em;
-                a.mo.v_scale[j / kOptBlock] = (uint8_t)er;
-            }
+    } else {
+#pragma unroll 1
+        for (uint32_t i = tid * 4; i < c.np; i += 1024) {
+            if (i >= 1024) load_operands<BITS, PDT, GDT, FULL, NT>(c, i, d);
+            update<BITS, PDT, GDT, FULL, NT>(sc, sh, c, i, d);
         }
-        float x[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = fmaf(step, m[k] * __builtin_amdgcn_rcpf(fmaf(r[k], isb2, eps)), d.p[k] * decay);
-        if constexpr (PDT == 0) store_f32(pp, i, n, x);
-        else {
-            // bf16 by stochastic rounding: 16 random bits under the last kept one, the rest cut off.  (A NaN whose low bits the
-            // sum would carry out of is replaced by the plain one.)
-            unsigned short q[4];
-            if (__builtin_expect(__builtin_isunordered(x[0], x[1]) || __builtin_isunordered(x[2], x[3]), 0)) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = x[k] != x[k] ? __uint_as_float(0x7FC00000u) : x[k];
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) q[k] = (unsigned short)((__float_as_uint(x[k]) + (mix32(h[k] + kGold) >> 16)) >> 16);
-            store_u16(pp, i, n, q);
-        }
-        d = next;
     }
 }
 
-template <int BITS>
+template <int BITS, int PDT, int GDT, bool NT>
+__device__ inline void adamw_chunk_any(const AdamWArgs& a, const Chunk& c, StepScalars* shared)
+{
+    if (c.n == kOptChunk && c.lo + (kOptChunk - 1) >= c.lo) adamw_chunk<BITS, PDT, GDT, true, NT>(a, c, shared);
+    else adamw_chunk<BITS, PDT, GDT, false, NT>(a, c, shared);
+}
+
+template <int BITS, bool NT>
 __global__ __launch_bounds__(256) void adamw_many_kernel(const AdamWArgs a)
 {
-    __shared__ StepScalars sh;
+    __shared__ StepScalars shared;
     const OptChunk ck = a.mo.chunks[a.chunk0 + blockIdx.x];
     const uint64_t pw = a.p[ck.tensor - a.tensor0], gw = a.g[ck.tensor - a.tensor0];
     if (gw == 0) return;
     if (a.sc.found_inf && *a.sc.found_inf != 0.f) return;
     const int pdt = (int)(pw >> 48), gdt = (int)(gw >> 48);
-    const uint64_t base = (uint64_t)ck.index * kOptChunk;
-    void* pp = (void*)((pw & kAddrMask) + base * (pdt ? 2 : 4));
-    const void* gp = (const void*)((gw & kAddrMask) + base * (gdt ? 2 : 4));
+    const uint64_t base = (uint64_t)ck.index * kOptChunk, off = (uint64_t)ck.offset32 * kOptBlock;
+    const Chunk c{(void*)((pw & kAddrMask) + base * (pdt ? 2 : 4)), (const void*)((gw & kAddrMask) + base * (gdt ? 2 : 4)),
+                  (uint8_t*)a.mo.m + off * (BITS / 8), (uint8_t*)a.mo.v + off * (BITS / 8), a.mo.m_scale + ck.offset32, a.mo.v_scale + ck.offset32,
+                  ck.count, round_up_block(ck.count), (uint32_t)off, (uint32_t)off + (uint32_t)(off >> 32) * kGold};
     if (pdt == 0) {
-        if (gdt == 0) adamw_chunk<BITS, 0, 0>(a, ck, pp, gp, &sh);
-        else adamw_chunk<BITS, 0, 1>(a, ck, pp, gp, &sh);
+        if (gdt == 0) adamw_chunk_any<BITS, 0, 0, NT>(a, c, &shared);
+        else adamw_chunk_any<BITS, 0, 1, NT>(a, c, &shared);
     } else {
-        if (gdt == 0) adamw_chunk<BITS, 1, 0>(a, ck, pp, gp, &sh);
-        else adamw_chunk<BITS, 1, 1>(a, ck, pp, gp, &sh);
+        if (gdt == 0) adamw_chunk_any<BITS, 1, 0, NT>(a, c, &shared);
+        else adamw_chunk_any<BITS, 1, 1, NT>(a, c, &shared);
     }
 }
 
@@ -388,13 +468,6 @@ __device__ inline Found find_tensor(const OptTensors& ts, uint32_t blk)
     return Found{(const char*)(t.ptr & kAddrMask), t.numel_lo | (t.ptr >> 52) << 32, (int)(t.ptr >> 48) & 15, blk - t.block0};
 }
 
-__device__ inline void load_quad_dt(int dt, const void* base, uint64_t i, uint64_t n, float (&x)[4])
-{
-    if (dt == 0) Quad<0>::load(base, i, n, x);
-    else if (dt == 1) Quad<1>::load(base, i, n, x);
-    else Quad<2>::load(base, i, n, x);
-}
-
 // ---- total norm --------------------------------------------------------------------------------------------------------
 __device__ inline double wave_sum(double x)
 {
@@ -413,10 +486,11 @@ struct Vec16 {
         f4 f;
         h8 h;
     };
+    template <bool NT>
     __device__ inline void load(const void* p, uint64_t i)
     {
-        if constexpr (DT == 0) f = *(const GLOBAL f4*)((const GLOBAL float*)p + i);
-        else h = *(const GLOBAL h8*)((const GLOBAL unsigned short*)p + i);
+        if constexpr (DT == 0) f = load_as<NT>((const GLOBAL f4*)((const GLOBAL float*)p + i));
+        else h = load_as<NT>((const GLOBAL h8*)((const GLOBAL unsigned short*)p + i));
     }
     __device__ inline double add(double acc) const
     {
@@ -429,7 +503,7 @@ struct Vec16 {
     }
 };
 
-template <int DT>
+template <int DT, bool NT>
 __device__ inline double sum_squares(const void* p, uint64_t base, uint64_t end)
 {
     constexpr int N = Vec16<DT>::N, U = 4;                 // four loads of 16 bytes requested before the first is used
@@ -439,14 +513,14 @@ __device__ inline double sum_squares(const void* p, uint64_t base, uint64_t end)
     for (; i + (U - 1) * STEP + N <= end; i += U * STEP) {
         Vec16<DT> x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u].load(p, i + u * STEP);
+        for (int u = 0; u < U; ++u) x[u].template load<NT>(p, i + u * STEP);
 #pragma unroll
         for (int u = 0; u < U; ++u) acc = x[u].add(acc);
     }
     for (; i < end; i += STEP) {
         if (i + N <= end) {
             Vec16<DT> x;
-            x.load(p, i);
+            x.template load<NT>(p, i);
             acc = x.add(acc);
         } else {
             for (uint64_t k = i; k < end; ++k) {
@@ -461,13 +535,16 @@ __device__ inline double sum_squares(const void* p, uint64_t base, uint64_t end)
 }
 
 // sums of squares in 64 bits, in a fixed order: one partial sum for each workgroup's elements
+template <bool NT>
 __global__ __launch_bounds__(256) void norm_partial_kernel(const OptTensors ts, uint32_t per_block, double* __restrict__ partial)
 {
     __shared__ double red[4];
     const Found f = find_tensor(ts, blockIdx.x);
     const uint64_t base = (uint64_t)f.block * per_block;
     const uint64_t end = base + per_block < f.n ? base + per_block : f.n;
-    double acc = f.dt == 0 ? sum_squares<0>(f.base, base, end) : f.dt == 1 ? sum_squares<1>(f.base, base, end) : sum_squares<2>(f.base, base, end);
+    double acc = f.dt == 0 ? sum_squares<0, NT>(f.base, base, end)
+               : f.dt == 1 ? sum_squares<1, NT>(f.base, base, end)
+                           : sum_squares<2, NT>(f.base, base, end);
     acc = wave_sum(acc);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
     __syncthreads();
@@ -501,24 +578,23 @@ __global__ __launch_bounds__(256) void scale_many_kernel(const OptTensors ts, co
     const float c = *coef;
     if (c == 1.f) return;
     const Found f = find_tensor(ts, blockIdx.x);
-    const uint64_t n = f.n;
-    const int dt = f.dt;
-    void* const q0 = (void*)f.base;
-    const uint64_t base = (uint64_t)f.block * kOptChunk;
-    for (int it = 0; it < kOptChunk / 1024; ++it) {
-        const uint64_t i = base + it * 1024 + threadIdx.x * 4;
-        if (i >= n) break;
+    const uint64_t base = (uint64_t)f.block * kOptChunk, left = f.n - base;
+    const uint32_t n = left < kOptChunk ? (uint32_t)left : kOptChunk;
+    void* const q0 = (void*)(f.base + base * (f.dt == 0 ? 4 : 2));
+    for (uint32_t i = threadIdx.x * 4; i < n; i += 1024) {
         float g[4];
-        load_quad_dt(dt, q0, i, n, g);
+        if (f.dt == 0) load_quad<0, false, false>(q0, i, n).values(g);
+        else if (f.dt == 1) load_quad<1, false, false>(q0, i, n).values(g);
+        else load_quad<2, false, false>(q0, i, n).values(g);
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[k] *= c;
-        if (dt == 0) store_f32(q0, i, n, g);
+        if (f.dt == 0) store_f32<false, false>(q0, i, n, g);
         else {
             unsigned short q[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                q[k] = dt == 1 ? bf16_nearest(g[k]) : __builtin_bit_cast(unsigned short, (_Float16)g[k]);
-            store_u16(q0, i, n, q);
+                q[k] = f.dt == 1 ? bf16_nearest(g[k]) : __builtin_bit_cast(unsigned short, (_Float16)g[k]);
+            store_u16<false, false>(q0, i, n, q);
         }
     }
 }
@@ -529,19 +605,21 @@ __global__ __launch_bounds__(256) void moments_pack_kernel(const float* __restri
                                                            uint8_t* __restrict__ m8, uint8_t* __restrict__ me, uint8_t* __restrict__ r8,
                                                            uint8_t* __restrict__ re)
 {
-    const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= ((n + kOptBlock - 1) & ~(uint64_t)(kOptBlock - 1))) return;
+    const uint64_t base = (uint64_t)blockIdx.x * 1024, left = n - base;
+    const uint32_t nb = left < 1024 ? (uint32_t)left : 1024, i = threadIdx.x * 4;
+    if (i >= round_up_block(nb)) return;
     float a[4], v4[4], b[4];
-    Quad<0>::load(m, i, n, a);
-    Quad<0>::load(v, i, n, v4);
-    roots(v4, b);
-    const uint32_t em = block_scale(a), er = block_scale(b);
+    const Quad<0> qm = load_quad<0, false, true>(m + base, i, nb), qv = load_quad<0, false, true>(v + base, i, nb);
+    qm.values(a);
+    qv.values(v4);
+    const bool plain = roots(v4, b);
+    const uint32_t em = block_scale<false>(a), er = block_scale<true>(b);
     const uint32_t half[4] = {0x80000000u, 0x80000000u, 0x80000000u, 0x80000000u};
-    *(uint32_t*)(m8 + i) = e4m3_codes<false>(a, em, half);
-    *(uint32_t*)(r8 + i) = e4m3_codes<true>(b, er, half);
-    if ((threadIdx.x & 7) == 0) {
-        me[i / kOptBlock] = (uint8_t)em;
-        re[i / kOptBlock] = (uint8_t)er;
+    *(uint32_t*)(m8 + base + i) = e4m3_codes(a, em, half);
+    *(uint32_t*)(r8 + base + i) = e4m3_root_codes(b, plain, er, half);
+    if ((i & 31) == 0) {
+        me[(base + i) / kOptBlock] = (uint8_t)em;
+        re[(base + i) / kOptBlock] = (uint8_t)er;
     }
 }
 
@@ -549,31 +627,34 @@ __global__ __launch_bounds__(256) void moments_unpack_kernel(const uint8_t* __re
                                                              const uint8_t* __restrict__ r8, const uint8_t* __restrict__ re,
                                                              float* __restrict__ m, float* __restrict__ v, uint64_t n)
 {
-    const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
+    const uint64_t base = (uint64_t)blockIdx.x * 1024, left = n - base;
+    const uint32_t nb = left < 1024 ? (uint32_t)left : 1024, i = threadIdx.x * 4;
+    if (i >= nb) return;
     float a[4], b[4];
-    e4m3_values(*(const uint32_t*)(m8 + i), me[i / kOptBlock], a);
-    e4m3_values(*(const uint32_t*)(r8 + i), re[i / kOptBlock], b);
+    e4m3_values(*(const uint32_t*)(m8 + base + i), me[(base + i) / kOptBlock], a);
+    e4m3_values(*(const uint32_t*)(r8 + base + i), re[(base + i) / kOptBlock], b);
 #pragma unroll
     for (int k = 0; k < 4; ++k) b[k] *= b[k];
-    store_f32(m, i, n, a);
-    store_f32(v, i, n, b);
+    store_f32<false, true>(m + base, i, nb, a);
+    store_f32<false, true>(v + base, i, nb, b);
 }
 
 }  // namespace
 
 uint32_t opt_mix(uint32_t x) { return mix32(x); }
 
-hipError_t launch_adamw_many(const AdamWArgs& a, int bits, uint32_t blocks, hipStream_t s)
+hipError_t launch_adamw_many(const AdamWArgs& a, int bits, bool streaming, uint32_t blocks, hipStream_t s)
 {
-    if (bits == 32) hipLaunchKernelGGL(adamw_many_kernel<32>, dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(adamw_many_kernel<8>, dim3(blocks), dim3(256), 0, s, a);
+    auto* k = bits == 32 ? (streaming ? adamw_many_kernel<32, true> : adamw_many_kernel<32, false>)
+                         : (streaming ? adamw_many_kernel<8, true> : adamw_many_kernel<8, false>);
+    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
-hipError_t launch_norm_partial(const OptTensors& ts, uint32_t blocks, uint32_t per_block, double* partial, hipStream_t s)
+hipError_t launch_norm_partial(const OptTensors& ts, bool streaming, uint32_t blocks, uint32_t per_block, double* partial, hipStream_t s)
 {
-    hipLaunchKernelGGL(norm_partial_kernel, dim3(blocks), dim3(256), 0, s, ts, per_block, partial);
+    auto* k = streaming ? norm_partial_kernel<true> : norm_partial_kernel<false>;
+    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, s, ts, per_block, partial);
     return hipGetLastError();
 }
 

@@ -576,6 +576,27 @@ def test_positions_that_pass_32_bits(bits):
     assert not after[4096:1 << 20].any()
 
 
+def test_a_chunk_that_crosses_the_32_bit_position():
+    """The second tensor starts at position 32: one of its chunks has elements on both sides of position 2^32."""
+    from superresolution_amd import optim
+    n = (1 << 32) + 5000
+    q, p, g = (torch.zeros(k, device="cuda", dtype=torch.bfloat16) for k in (7, n, n))
+    lo = (1 << 32) - 32 - 4064 - 4096                                   # 32 + lo is the start of a chunk, two before the crossing one
+    p[lo:], g[lo:] = _hash_floats(n - lo, 1, 0.1).cuda().bfloat16(), _hash_floats(n - lo, 2, 1e-2).cuda().bfloat16()
+    params = [torch.nn.Parameter(q), torch.nn.Parameter(p)]
+    params[0].grad, params[1].grad = torch.ones_like(q), g
+    opt = optim.AdamW(params, lr=1e-2, state_bits=8, seed=9)
+    ref = R.AdamWRef(_f64(p[lo:]), bits=8, lr=1e-2, seed=9, bf16=True, offset=32, first=lo)
+    opt.step()
+    ref.step(_f64(g[lo:]))
+    k = R.padded(n - lo)
+    np.testing.assert_array_equal(_f64(opt.moments[0].exp_avg[32 + lo:32 + lo + k].float()), ref.m8[0])
+    np.testing.assert_array_equal(_f64(opt.moments[0].root[32 + lo:32 + lo + k].float()), ref.r8[0])
+    a, b = ref.ends
+    got = _f64(params[1][lo:])
+    assert ((got >= np.minimum(a, b)) & (got <= np.maximum(a, b))).all()
+
+
 # ---- total norm, clipping ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("sizes", list(SIZES))
