@@ -5,13 +5,28 @@
 namespace srgen {
 namespace {
 
+// an address that came as a number is in device memory: without this it would be reached by flat loads
+#define GLOBAL __attribute__((address_space(1)))
+
 // unaligned vectors: a gradient that is a view into a flat buffer starts at any element (global loads need element alignment only)
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
-typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
-// an address that came as a number is in device memory: without this it would be reached by flat loads
-#define GLOBAL __attribute__((address_space(1)))
+template <int V>
+struct HalfVec;
+template <>
+struct HalfVec<4> {
+    typedef unsigned short type __attribute__((ext_vector_type(4)));
+    typedef unsigned short unaligned __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t codes __attribute__((ext_vector_type(1), aligned(4)));
+};
+template <>
+struct HalfVec<8> {
+    typedef unsigned short type __attribute__((ext_vector_type(8)));
+    typedef unsigned short unaligned __attribute__((ext_vector_type(8), aligned(2)));
+    typedef uint32_t codes __attribute__((ext_vector_type(2), aligned(4)));
+};
+template <int V>
+using Codes = typename HalfVec<V>::codes;      // V e4m3 values, four to a word
 
 constexpr uint32_t kGold = 0x9E3779B9u;        // 2^32 / golden ratio: consecutive steps and high words get far keys
 
@@ -41,84 +56,84 @@ __device__ inline void store_as(T x, GLOBAL T* p)
     else *p = x;
 }
 
-// Four consecutive elements as they are in memory (values() converts: a conversion beside the load would wait for it).
+// V consecutive elements as they are in memory (values() converts: a conversion beside the load would wait for it).
 // DT: 0 fp32, 1 bf16, 2 fp16.
-template <int DT>
-struct Quad {
-    u16x4 h;
-    __device__ inline void values(float (&x)[4]) const
+template <int DT, int V>
+struct Elements {
+    typename HalfVec<V>::type h;
+    __device__ inline void values(float (&x)[V]) const
     {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < V; ++k)
             x[k] = DT == 1 ? bf16_to_f32(h[k]) : (float)__builtin_bit_cast(_Float16, (unsigned short)h[k]);
     }
 };
-template <>
-struct Quad<0> {
-    f32x4 f;
-    __device__ inline void values(float (&x)[4]) const
+template <int V>
+struct Elements<0, V> {
+    f32x4 f[V / 4];
+    __device__ inline void values(float (&x)[V]) const
     {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = f[k];
+        for (int k = 0; k < V; ++k) x[k] = f[k / 4][k % 4];
     }
 };
 
-// elements i .. i + 3 of `n`; behind the end: zeros.  FULL: all four are there.  The index counts from a base that is the same
-// for the workgroup, in 32 bits.
-template <int DT, bool FULL, bool NT>
-__device__ inline Quad<DT> load_quad(const void* base, uint32_t i, uint32_t n)
+// elements i .. i + V - 1 of `n`; behind the end: zeros.  FULL: all are there.  The index counts from a base that is the same for
+// the workgroup, in 32 bits.
+template <int DT, int V, bool FULL, bool NT>
+__device__ inline Elements<DT, V> load_elements(const void* base, uint32_t i, uint32_t n)
 {
-    Quad<DT> a;
+    Elements<DT, V> a;
     if constexpr (DT == 0) {
         const GLOBAL float* q = (const GLOBAL float*)base + i;
-        if (!FULL) a.f = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (FULL || i + 4 <= n) a.f = load_as<NT>((const GLOBAL f32x4u*)q);
-        else if (i < n) {
-            a.f[0] = q[0];
-            if (i + 1 < n) a.f[1] = q[1];
-            if (i + 2 < n) a.f[2] = q[2];
+#pragma unroll
+        for (int u = 0; u < V / 4; ++u) {
+            if (!FULL) a.f[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const uint32_t at = i + 4 * u;
+            if (FULL || at + 4 <= n) a.f[u] = load_as<NT>((const GLOBAL f32x4u*)(q + 4 * u));
+            else if (at < n) {
+                a.f[u][0] = q[4 * u];
+                if (at + 1 < n) a.f[u][1] = q[4 * u + 1];
+                if (at + 2 < n) a.f[u][2] = q[4 * u + 2];
+            }
         }
     } else {
         const GLOBAL unsigned short* q = (const GLOBAL unsigned short*)base + i;
-        if (!FULL) a.h = u16x4{0, 0, 0, 0};
-        if (FULL || i + 4 <= n) a.h = load_as<NT>((const GLOBAL u16x4u*)q);
-        else if (i < n) {
-            a.h[0] = q[0];
-            if (i + 1 < n) a.h[1] = q[1];
-            if (i + 2 < n) a.h[2] = q[2];
+        if (FULL || i + V <= n) a.h = load_as<NT>((const GLOBAL typename HalfVec<V>::unaligned*)q);
+        else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) a.h[k] = i + k < n ? q[k] : (unsigned short)0;
         }
     }
     return a;
 }
 
-template <bool FULL, bool NT>
-__device__ inline void store_f32(void* base, uint32_t i, uint32_t n, const float (&x)[4])
+template <int V, bool FULL, bool NT>
+__device__ inline void store_f32(void* base, uint32_t i, uint32_t n, const float (&x)[V])
 {
     GLOBAL float* q = (GLOBAL float*)base + i;
-    if (FULL || i + 4 <= n) {
-        f32x4u a;
+    if (FULL || i + V <= n) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = x[k];
-        store_as<NT>(a, (GLOBAL f32x4u*)q);
+        for (int u = 0; u < V / 4; ++u) store_as<NT>(f32x4u{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]}, (GLOBAL f32x4u*)(q + 4 * u));
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < V; ++k)
             if (i + k < n) q[k] = x[k];
     }
 }
 
-template <bool FULL, bool NT>
-__device__ inline void store_u16(void* base, uint32_t i, uint32_t n, const unsigned short (&x)[4])
+template <int V, bool FULL, bool NT>
+__device__ inline void store_u16(void* base, uint32_t i, uint32_t n, const unsigned short (&x)[V])
 {
     GLOBAL unsigned short* q = (GLOBAL unsigned short*)base + i;
-    if (FULL || i + 4 <= n) {
-        u16x4u a;
+    if (FULL || i + V <= n) {
+        typename HalfVec<V>::unaligned a;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = x[k];
-        store_as<NT>(a, (GLOBAL u16x4u*)q);
+        for (int k = 0; k < V; ++k) a[k] = x[k];
+        store_as<NT>(a, (GLOBAL typename HalfVec<V>::unaligned*)q);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < V; ++k)
             if (i + k < n) q[k] = x[k];
     }
 }
@@ -138,12 +153,7 @@ __device__ inline unsigned short bf16_nearest(float x)
 // random bits at the top of the seed it gave the definition's code for all of 4 million values, seeds and scales tried,
 // subnormals, ties, infinities and NaN among them.  v_cvt_scalef32_pk_f32_fp8 reads two values back, all 256 scales right.
 constexpr uint32_t kTop = 0x7F600000u;         // 1.75 * 2^127: what is above is stored as it, or it would round up to infinity
-
-__device__ inline uint32_t scale_byte(uint32_t top_bits)
-{
-    const uint32_t e = (top_bits + 0x1FFFFFu) >> 23;
-    return (e < 9u ? 9u : e) - 8u;
-}
+constexpr uint32_t kLow = (9u << 23) - 0x1FFFFFu;  // a maximum below this counts as this: the scale is then 2^-126, the lowest
 
 __device__ inline uint32_t finite_bits(float x)
 {
@@ -157,94 +167,119 @@ __device__ inline uint32_t max_dpp(uint32_t x)
     const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false);   // (0: one instruction with the max)
     return x > o ? x : o;
 }
-__device__ inline uint32_t max8(uint32_t x)                  // over the 8 lanes that hold one block: neighbours, pairs, the two quads
+// over the 32 / V lanes that hold one block: neighbours, pairs and, of 8, the two quads
+template <int V>
+__device__ inline uint32_t max_block(uint32_t x)
 {
-    return max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(x)));  // quad_perm [1,0,3,2], quad_perm [2,3,0,1], row_half_mirror
+    x = max_dpp<0x4E>(max_dpp<0xB1>(x));                     // quad_perm [1,0,3,2], quad_perm [2,3,0,1]
+    return V == 4 ? max_dpp<0x141>(x) : x;                   // row_half_mirror
 }
 
-// The scale byte of a block whose lane holds x[0..3]; magnitudes above kTop are brought down to it, in a branch that is hardly
-// ever taken (v_max skips NaN; in a root's bits NaN is above everything).  ROOT: no x is negative.
-template <bool ROOT>
-__device__ inline uint32_t block_scale(float (&x)[4])
+__device__ inline uint32_t max_u32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// The scale (as a float's bits) of a block whose lane holds x[0 .. V-1]; magnitudes above kTop are brought down to it, in a branch
+// that is hardly ever taken (v_max skips NaN; in a root's bits NaN is above everything).  ROOT: no x is negative.
+template <int V, bool ROOT>
+__device__ inline uint32_t block_scale(float (&x)[V])
 {
     uint32_t t;
     if constexpr (ROOT) {
-        const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]), c = __float_as_uint(x[2]), d = __float_as_uint(x[3]);
-        const uint32_t ab = a > b ? a : b, cd = c > d ? c : d;
-        t = ab > cd ? ab : cd;
-    } else t = __float_as_uint(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-    uint32_t top = max8(t);
-    if (__builtin_expect(top > kTop, 0)) {                   // (the same in all 8 lanes)
-        uint32_t b = 0;
+        t = kLow;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; k += 2) t = max_u32(max_u32(t, __float_as_uint(x[k])), __float_as_uint(x[k + 1]));
+    } else {
+        float f = __uint_as_float(kLow);
+#pragma unroll
+        for (int k = 0; k < V; k += 2) f = fmaxf(fmaxf(f, fabsf(x[k])), fabsf(x[k + 1]));
+        t = __float_as_uint(f);
+    }
+    uint32_t top = max_block<V>(t);
+    if (__builtin_expect(top > kTop, 0)) {                   // (the same in all lanes of the block)
+        uint32_t b = kLow;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
             const uint32_t f = finite_bits(x[k]);
             if (f == kTop) x[k] = copysignf(__uint_as_float(kTop), x[k]);
-            b = b > f ? b : f;
+            b = max_u32(b, f);
         }
-        top = max8(b);
+        top = max_block<V>(b);
     }
-    return scale_byte(top);
+    return ((top + 0x1FFFFFu) & 0x7F800000u) - (8u << 23);
 }
 
-// four codes
-__device__ inline uint32_t e4m3_codes(const float (&x)[4], uint32_t e, const uint32_t (&seed)[4])
+template <int V>
+__device__ inline Codes<V> e4m3_codes(const float (&x)[V], uint32_t scale, const uint32_t (&seed)[V])
 {
-    const float s = __uint_as_float(e << 23);
-    int c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[0], seed[0], s, 0);
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[1], seed[1], s, 1);
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[2], seed[2], s, 2);
-    c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[3], seed[3], s, 3);
-    return (uint32_t)c;
+    const float s = __uint_as_float(scale);
+    Codes<V> out;
+#pragma unroll
+    for (int u = 0; u < V; u += 4) {
+        int c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[u], seed[u], s, 0);
+        c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[u + 1], seed[u + 1], s, 1);
+        c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[u + 2], seed[u + 2], s, 2);
+        c = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(c, x[u + 3], seed[u + 3], s, 3);
+        out[u / 4] = (uint32_t)c;
+    }
+    return out;
 }
 
 // the same for roots: what is not zero is raised to the smallest code, 2^-9 of the scale.  `plain`: none is 0 or NaN (roots())
-__device__ inline uint32_t e4m3_root_codes(const float (&x)[4], bool plain, uint32_t e, const uint32_t (&seed)[4])
+template <int V>
+__device__ inline Codes<V> e4m3_root_codes(const float (&x)[V], bool plain, uint32_t scale, const uint32_t (&seed)[V])
 {
-    const float q = __uint_as_float(e << 23) * 0x1p-9f;
-    float y[4];
+    const float q = __uint_as_float(scale) * 0x1p-9f;
+    float y[V];
     if (__builtin_expect(plain, 1)) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {                        // (as whole numbers: the same order, and no care for NaN)
-            const uint32_t a = __float_as_uint(x[k]), b = __float_as_uint(q);
-            y[k] = __uint_as_float(a > b ? a : b);
-        }
+        for (int k = 0; k < V; ++k) y[k] = __uint_as_float(max_u32(__float_as_uint(x[k]), __float_as_uint(q)));  // (whole numbers: no care for NaN)
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = x[k] > 0.f && x[k] < q ? q : x[k];
+        for (int k = 0; k < V; ++k) y[k] = x[k] > 0.f && x[k] < q ? q : x[k];
     }
-    return e4m3_codes(y, e, seed);
+    return e4m3_codes<V>(y, scale, seed);
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-__device__ inline void e4m3_values(uint32_t c, uint32_t e, float (&x)[4])
+template <int V>
+__device__ inline void e4m3_values(Codes<V> c, uint32_t e, float (&x)[V])
 {
     const float s = __uint_as_float(e << 23);                // (the instruction reads 0 as 2^-127 and 255 as NaN, as e8m0 does)
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, s, true);
-    x[0] = a[0];
-    x[1] = a[1];
-    x[2] = b[0];
-    x[3] = b[1];
+#pragma unroll
+    for (int u = 0; u < V; u += 4) {
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[u / 4], s, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[u / 4], s, true);
+        x[u] = a[0];
+        x[u + 1] = a[1];
+        x[u + 2] = b[0];
+        x[u + 3] = b[1];
+    }
 }
 
 // Square roots to the nearest: y ~ 1 / sqrt(v), s = v y, then the residual v - s^2, exact in one fma, put right with y / 2.
 // That is within 2^-45 of the root before the last rounding.  Below 2^-90 (the residual would underflow), at 0, infinity and NaN
 // sqrtf instead; returns whether there was none of these.
-__device__ inline bool roots(const float (&v)[4], float (&r)[4])
+template <int V>
+__device__ inline bool roots(const float (&v)[V], float (&r)[V])
 {
-    const float lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), hi = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-    const bool plain = lo >= 0x1p-90f && hi < INFINITY && !__builtin_isunordered(v[0], v[1]) && !__builtin_isunordered(v[2], v[3]);
+    float lo = v[0], hi = v[0];
+    bool plain = true;
+#pragma unroll
+    for (int k = 0; k < V; k += 2) {
+        lo = fminf(fminf(lo, v[k]), v[k + 1]);
+        hi = fmaxf(fmaxf(hi, v[k]), v[k + 1]);
+        plain = plain && !__builtin_isunordered(v[k], v[k + 1]);
+    }
+    plain = plain && lo >= 0x1p-90f && hi < INFINITY;
     if (__builtin_expect(plain, 1)) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; ++k) {
             const float y = __builtin_amdgcn_rsqf(v[k]);
             const float s = v[k] * y;
             r[k] = fmaf(fmaf(-s, s, v[k]), 0.5f * y, s);
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) r[k] = sqrtf(v[k]);
+        for (int k = 0; k < V; ++k) r[k] = sqrtf(v[k]);
     }
     return plain;
 }
@@ -253,21 +288,26 @@ __device__ inline bool roots(const float (&v)[4], float (&r)[4])
 //   g' = c g      m = b1 m + (1 - b1) g'      v = b2 v + (1 - b2) g'^2
 //   p  = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // One workgroup owns kOptChunk consecutive elements of one tensor and that chunk's step counter, so t needs no second launch
-// and no atomics: every chunk of a tensor counts the same steps.  All loads of the chunk are requested first; meanwhile one wave
-// works out the step's scalars (two exponentials, divisions and a root in 64 bits) and hands them over through LDS.
+// and no atomics: every chunk of a tensor counts the same steps.  The first loads are requested before anything else; meanwhile
+// one wave works out the step's scalars (two exponentials, divisions and a root in 64 bits) and hands them over through LDS.
+// A thread takes V elements at a time: 4, or 8 of bf16 with 8-bit moments, where the arithmetic is what takes the time and half
+// as many threads to a block of 32 make its scale cheaper.
 struct StepScalars {
     double c1, c2;          // (1 - beta1) * c, (1 - beta2) * c^2
-    float decay, step, isb2, gmul;
+    float decay;            // 1 - lr wd
+    float ra, rb;           // p - m / (ra r + rb): 1 / (s sqrt(1 - b2^t)) and eps / s with the step size s = lr / (1 - b1^t)
+    float gmul;
     uint32_t key;
 };
 
-// what a thread reads for its four elements
-template <int BITS, int PDT, int GDT>
+// what a thread reads for its V elements
+template <int BITS, int PDT, int GDT, int V>
 struct Operands {
-    Quad<PDT> p;
-    Quad<GDT> g;
-    f32x4 m, v;                        // 32 bits
-    uint32_t mc, vc, me, ve;           // 8 bits
+    Elements<PDT, V> p;
+    Elements<GDT, V> g;
+    Elements<0, V> m, v;               // 32 bits
+    Codes<V> mc, vc;                   // 8 bits
+    uint32_t me, ve;
 };
 
 // a chunk's operands: bases are the same for the workgroup, indexes count from them
@@ -278,37 +318,37 @@ struct Chunk {
     uint8_t* v;
     uint8_t* me;
     uint8_t* ve;
-    uint32_t n, np;                    // elements; the same in whole blocks of 32 (8 lanes)
+    uint32_t n, np;                    // elements; the same in whole blocks of 32
     uint32_t lo, w;                    // position: its low word; that with the high word mixed in
 };
 
-template <int BITS, int PDT, int GDT, bool FULL, bool NT>
-__device__ inline void load_operands(const Chunk& c, uint32_t i, Operands<BITS, PDT, GDT>& d)
+template <int BITS, int PDT, int GDT, int V, bool FULL, bool NT>
+__device__ inline void load_operands(const Chunk& c, uint32_t i, Operands<BITS, PDT, GDT, V>& d)
 {
-    d.p = load_quad<PDT, FULL, NT>(c.p, i, c.n);
-    d.g = load_quad<GDT, FULL, NT>(c.g, i, c.n);
+    d.p = load_elements<PDT, V, FULL, NT>(c.p, i, c.n);
+    d.g = load_elements<GDT, V, FULL, NT>(c.g, i, c.n);
     if constexpr (BITS == 32) {
-        if (!FULL) d.m = d.v = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (FULL || i < c.np) {
-            d.m = load_as<NT>((const GLOBAL f32x4*)(c.m + i * 4));
-            d.v = load_as<NT>((const GLOBAL f32x4*)(c.v + i * 4));
-        }
+        d.m = load_elements<0, V, FULL, NT>(c.m, i, c.np);
+        d.v = load_elements<0, V, FULL, NT>(c.v, i, c.np);
     } else {
-        if (!FULL) d.mc = d.vc = d.me = d.ve = 0;
+        if (!FULL) {
+            d.mc = d.vc = 0;
+            d.me = d.ve = 0;
+        }
         if (FULL || i < c.np) {
-            d.mc = load_as<NT>((const GLOBAL uint32_t*)(c.m + i));
-            d.vc = load_as<NT>((const GLOBAL uint32_t*)(c.v + i));
+            d.mc = load_as<NT>((const GLOBAL Codes<V>*)(c.m + i));
+            d.vc = load_as<NT>((const GLOBAL Codes<V>*)(c.v + i));
             d.me = ((const GLOBAL uint8_t*)c.me)[i / kOptBlock];
             d.ve = ((const GLOBAL uint8_t*)c.ve)[i / kOptBlock];
         }
     }
 }
 
-template <int BITS, int PDT, int GDT, bool FULL, bool NT>
-__device__ inline void update(const AdamWScalars& sc, const StepScalars& sh, const Chunk& c, uint32_t i, Operands<BITS, PDT, GDT>& d)
+template <int BITS, int PDT, int GDT, int V, bool FULL, bool NT>
+__device__ inline void update(const AdamWScalars& sc, const StepScalars& sh, const Chunk& c, uint32_t i, const Operands<BITS, PDT, GDT, V>& d)
 {
-    float m[4], r[4], p[4], g[4];
-    uint32_t h[4];
+    float m[V], r[V], p[V], g[V];
+    uint32_t h[V];
     bool plain = true;
     d.g.values(g);
     d.p.values(p);
@@ -316,62 +356,66 @@ __device__ inline void update(const AdamWScalars& sc, const StepScalars& sh, con
         uint32_t w = c.w + i;
         if (!FULL && c.lo + i < c.lo) w += kGold;                      // (the high word goes up inside the chunk)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = mix32((w + k) ^ sh.key);
+        for (int k = 0; k < V; ++k) h[k] = mix32((w + k) ^ sh.key);
     }
     if constexpr (BITS == 32) {
         const float b1 = (float)sc.beta1, d1 = (float)(1.0 - sc.beta1), b2 = (float)sc.beta2, d2 = (float)(1.0 - sc.beta2);
+        float v[V];
+        d.m.values(m);
+        d.v.values(v);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; ++k) {
             const float gk = g[k] * sh.gmul;
-            d.m[k] = fmaf(b1, d.m[k], d1 * gk);
-            d.v[k] = fmaf(b2, d.v[k], (d2 * gk) * gk);
-            m[k] = d.m[k];
-            r[k] = sqrtf(d.v[k]);
+            m[k] = fmaf(b1, m[k], d1 * gk);
+            v[k] = fmaf(b2, v[k], (d2 * gk) * gk);
+            r[k] = sqrtf(v[k]);
         }
-        store_as<NT>(d.m, (GLOBAL f32x4*)(c.m + i * 4));
-        store_as<NT>(d.v, (GLOBAL f32x4*)(c.v + i * 4));
+        store_f32<V, true, NT>(c.m, i, 0, m);                          // (the padding of the last block is there)
+        store_f32<V, true, NT>(c.v, i, 0, v);
     } else {
-        float mo[4], ro[4], v[4];
-        e4m3_values(d.mc, d.me, mo);
-        e4m3_values(d.vc, d.ve, ro);
+        float mo[V], ro[V], v[V];
+        e4m3_values<V>(d.mc, d.me, mo);
+        e4m3_values<V>(d.vc, d.ve, ro);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; ++k) {
             const double gk = (double)g[k], rk = (double)ro[k];
             m[k] = (float)fma(sc.beta1, (double)mo[k], sh.c1 * gk);
             v[k] = (float)fma(sc.beta2, rk * rk, sh.c2 * (gk * gk));
         }
-        plain = roots(v, r);
+        plain = roots<V>(v, r);
     }
-    float x[4];
-    const float step = -sh.step, eps = (float)sc.eps;
+    float x[V];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = fmaf(step, m[k] * __builtin_amdgcn_rcpf(fmaf(r[k], sh.isb2, eps)), p[k] * sh.decay);
-    if constexpr (PDT == 0) store_f32<FULL, NT>(c.p, i, c.n, x);
+    for (int k = 0; k < V; ++k) x[k] = fmaf(-m[k], __builtin_amdgcn_rcpf(fmaf(r[k], sh.ra, sh.rb)), p[k] * sh.decay);
+    if constexpr (PDT == 0) store_f32<V, FULL, NT>(c.p, i, c.n, x);
     else {
         // bf16 by stochastic rounding: 16 random bits under the last kept one, the rest cut off.  (A NaN whose low bits the sum
         // would carry out of is replaced by the plain one.)
-        unsigned short q[4];
-        if (__builtin_expect(__builtin_isunordered(x[0], x[1]) || __builtin_isunordered(x[2], x[3]), 0)) {
+        unsigned short q[V];
+        bool nan = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = x[k] != x[k] ? __uint_as_float(0x7FC00000u) : x[k];
+        for (int k = 0; k < V; k += 2) nan = nan || __builtin_isunordered(x[k], x[k + 1]);
+        if (__builtin_expect(nan, 0)) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[k] = x[k] != x[k] ? __uint_as_float(0x7FC00000u) : x[k];
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = (unsigned short)((__float_as_uint(x[k]) + (mix32(h[k] + kGold) >> 16)) >> 16);
-        store_u16<FULL, NT>(c.p, i, c.n, q);
+        for (int k = 0; k < V; ++k) q[k] = (unsigned short)((__float_as_uint(x[k]) + (mix32(h[k] + kGold) >> 16)) >> 16);
+        store_u16<V, FULL, NT>(c.p, i, c.n, q);
     }
     if constexpr (BITS == 8) {
-        uint32_t seed_m[4], seed_r[4];
+        uint32_t seed_m[V], seed_r[V];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < V; ++k) {
             seed_m[k] = h[k] << 16;
             seed_r[k] = h[k] & 0xFFFF0000u;
         }
-        const uint32_t em = block_scale<false>(m), er = block_scale<true>(r);
-        store_as<NT>(e4m3_codes(m, em, seed_m), (GLOBAL uint32_t*)(c.m + i));
-        store_as<NT>(e4m3_root_codes(r, plain, er, seed_r), (GLOBAL uint32_t*)(c.v + i));
-        if ((threadIdx.x & 7) == 0) {
-            ((GLOBAL uint8_t*)c.me)[i / kOptBlock] = (uint8_t)em;
-            ((GLOBAL uint8_t*)c.ve)[i / kOptBlock] = (uint8_t)er;
+        const uint32_t em = block_scale<V, false>(m), er = block_scale<V, true>(r);
+        store_as<NT>(e4m3_codes<V>(m, em, seed_m), (GLOBAL Codes<V>*)(c.m + i));
+        store_as<NT>(e4m3_root_codes<V>(r, plain, er, seed_r), (GLOBAL Codes<V>*)(c.v + i));
+        if ((i & (kOptBlock - 1)) == 0) {
+            ((GLOBAL uint8_t*)c.me)[i / kOptBlock] = (uint8_t)(em >> 23);
+            ((GLOBAL uint8_t*)c.ve)[i / kOptBlock] = (uint8_t)(er >> 23);
         }
     }
 }
@@ -379,15 +423,18 @@ __device__ inline void update(const AdamWScalars& sc, const StepScalars& sh, con
 template <int BITS, int PDT, int GDT, bool FULL, bool NT>
 __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScalars* shared)
 {
+    constexpr int V = BITS == 8 && PDT == 1 && GDT == 1 ? 8 : 4;
+    constexpr uint32_t STRIDE = 256 * V;
     const AdamWScalars& sc = a.sc;
     const uint32_t tid = threadIdx.x;
-    Operands<BITS, PDT, GDT> d, next;
-    load_operands<BITS, PDT, GDT, FULL, NT>(c, tid * 4, d);
+    Operands<BITS, PDT, GDT, V> d, next;
+    load_operands<BITS, PDT, GDT, V, FULL, NT>(c, tid * V, d);
     if (tid < 64) {
         int32_t* counter = a.mo.step + (size_t)a.chunk0 + blockIdx.x;
         const int t = *counter + 1;                                    // (this wave alone reads and writes it)
         const double lr = sc.lr_dev ? (double)*sc.lr_dev : sc.lr;
         const double bc1 = -expm1((double)t * sc.ln_beta1), bc2 = -expm1((double)t * sc.ln_beta2);
+        const double s = lr / bc1;
         double f = sc.grad_mul ? (double)*sc.grad_mul : 1.0;
         if (sc.grad_div) f /= (double)*sc.grad_div;
         if (sc.negate) f = -f;
@@ -396,8 +443,9 @@ __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScala
             shared->c1 = (1.0 - sc.beta1) * f;
             shared->c2 = (1.0 - sc.beta2) * (f * f);
             shared->decay = (float)(1.0 - lr * sc.wd);
-            shared->step = (float)(lr / bc1);
-            shared->isb2 = (float)(1.0 / sqrt(bc2));
+            // (a step size of 0: an infinite denominator, without infinity times a root that is 0)
+            shared->ra = s == 0.0 ? 0.f : (float)(1.0 / (s * sqrt(bc2)));
+            shared->rb = s == 0.0 ? INFINITY : (float)(sc.eps / s);
             shared->gmul = (float)f;
             shared->key = mix32(sc.seed_key + (uint32_t)t * kGold);
         }
@@ -406,16 +454,16 @@ __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScala
     const StepScalars sh = *shared;
     if constexpr (FULL) {
 #pragma unroll 2
-        for (uint32_t i0 = 0; i0 < kOptChunk; i0 += 1024) {
-            if (i0 + 1024 < kOptChunk) load_operands<BITS, PDT, GDT, FULL, NT>(c, i0 + 1024 + tid * 4, next);
-            update<BITS, PDT, GDT, FULL, NT>(sc, sh, c, i0 + tid * 4, d);
+        for (uint32_t i0 = 0; i0 < kOptChunk; i0 += STRIDE) {
+            if (i0 + STRIDE < kOptChunk) load_operands<BITS, PDT, GDT, V, FULL, NT>(c, i0 + STRIDE + tid * V, next);
+            update<BITS, PDT, GDT, V, FULL, NT>(sc, sh, c, i0 + tid * V, d);
             d = next;
         }
     } else {
 #pragma unroll 1
-        for (uint32_t i = tid * 4; i < c.np; i += 1024) {
-            if (i >= 1024) load_operands<BITS, PDT, GDT, FULL, NT>(c, i, d);
-            update<BITS, PDT, GDT, FULL, NT>(sc, sh, c, i, d);
+        for (uint32_t i = tid * V; i < c.np; i += STRIDE) {
+            if (i >= STRIDE) load_operands<BITS, PDT, GDT, V, FULL, NT>(c, i, d);
+            update<BITS, PDT, GDT, V, FULL, NT>(sc, sh, c, i, d);
         }
     }
 }
@@ -583,18 +631,18 @@ __global__ __launch_bounds__(256) void scale_many_kernel(const OptTensors ts, co
     void* const q0 = (void*)(f.base + base * (f.dt == 0 ? 4 : 2));
     for (uint32_t i = threadIdx.x * 4; i < n; i += 1024) {
         float g[4];
-        if (f.dt == 0) load_quad<0, false, false>(q0, i, n).values(g);
-        else if (f.dt == 1) load_quad<1, false, false>(q0, i, n).values(g);
-        else load_quad<2, false, false>(q0, i, n).values(g);
+        if (f.dt == 0) load_elements<0, 4, false, false>(q0, i, n).values(g);
+        else if (f.dt == 1) load_elements<1, 4, false, false>(q0, i, n).values(g);
+        else load_elements<2, 4, false, false>(q0, i, n).values(g);
 #pragma unroll
         for (int k = 0; k < 4; ++k) g[k] *= c;
-        if (f.dt == 0) store_f32<false, false>(q0, i, n, g);
+        if (f.dt == 0) store_f32<4, false, false>(q0, i, n, g);
         else {
             unsigned short q[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
                 q[k] = f.dt == 1 ? bf16_nearest(g[k]) : __builtin_bit_cast(unsigned short, (_Float16)g[k]);
-            store_u16<false, false>(q0, i, n, q);
+            store_u16<4, false, false>(q0, i, n, q);
         }
     }
 }
@@ -609,17 +657,17 @@ __global__ __launch_bounds__(256) void moments_pack_kernel(const float* __restri
     const uint32_t nb = left < 1024 ? (uint32_t)left : 1024, i = threadIdx.x * 4;
     if (i >= round_up_block(nb)) return;
     float a[4], v4[4], b[4];
-    const Quad<0> qm = load_quad<0, false, true>(m + base, i, nb), qv = load_quad<0, false, true>(v + base, i, nb);
+    const Elements<0, 4> qm = load_elements<0, 4, false, true>(m + base, i, nb), qv = load_elements<0, 4, false, true>(v + base, i, nb);
     qm.values(a);
     qv.values(v4);
-    const bool plain = roots(v4, b);
-    const uint32_t em = block_scale<false>(a), er = block_scale<true>(b);
+    const bool plain = roots<4>(v4, b);
+    const uint32_t em = block_scale<4, false>(a), er = block_scale<4, true>(b);
     const uint32_t half[4] = {0x80000000u, 0x80000000u, 0x80000000u, 0x80000000u};
-    *(uint32_t*)(m8 + base + i) = e4m3_codes(a, em, half);
-    *(uint32_t*)(r8 + base + i) = e4m3_root_codes(b, plain, er, half);
+    *(Codes<4>*)(m8 + base + i) = e4m3_codes<4>(a, em, half);
+    *(Codes<4>*)(r8 + base + i) = e4m3_root_codes<4>(b, plain, er, half);
     if ((i & 31) == 0) {
-        me[(base + i) / kOptBlock] = (uint8_t)em;
-        re[(base + i) / kOptBlock] = (uint8_t)er;
+        me[(base + i) / kOptBlock] = (uint8_t)(em >> 23);
+        re[(base + i) / kOptBlock] = (uint8_t)(er >> 23);
     }
 }
 
@@ -631,12 +679,12 @@ __global__ __launch_bounds__(256) void moments_unpack_kernel(const uint8_t* __re
     const uint32_t nb = left < 1024 ? (uint32_t)left : 1024, i = threadIdx.x * 4;
     if (i >= nb) return;
     float a[4], b[4];
-    e4m3_values(*(const uint32_t*)(m8 + base + i), me[(base + i) / kOptBlock], a);
-    e4m3_values(*(const uint32_t*)(r8 + base + i), re[(base + i) / kOptBlock], b);
+    e4m3_values<4>(*(const Codes<4>*)(m8 + base + i), me[(base + i) / kOptBlock], a);
+    e4m3_values<4>(*(const Codes<4>*)(r8 + base + i), re[(base + i) / kOptBlock], b);
 #pragma unroll
     for (int k = 0; k < 4; ++k) b[k] *= b[k];
-    store_f32<false, true>(m + base, i, nb, a);
-    store_f32<false, true>(v + base, i, nb, b);
+    store_f32<4, false, true>(m + base, i, nb, a);
+    store_f32<4, false, true>(v + base, i, nb, b);
 }
 
 }  // namespace
