@@ -561,6 +561,10 @@ typedef struct srgen_adamw_args {
     const float* grad_mul;    /* device scalar the gradients are multiplied by (clip coefficient), or NULL      */
     const float* grad_div;    /* device scalar the gradients are divided by (loss scale), or NULL               */
     const float* found_inf;   /* device scalar: not zero = nothing happens, no counter moves; or NULL           */
+    float* norm_coef2;        /* not NULL: srgen_total_norm over the list's gradients comes first, the step clips by it */
+    void* norm_scratch;       /* (grad_mul is NULL then; max_norm, scratch and result as there)                   */
+    size_t norm_scratch_bytes;
+    double max_norm;
     uint32_t seed;            /* of the stochastic rounding */
     int32_t maximize;         /* 1: the gradients' sign is changed */
 } srgen_adamw_args;

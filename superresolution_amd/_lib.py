@@ -43,8 +43,9 @@ class srgen_moments(ctypes.Structure):
 class srgen_adamw_args(ctypes.Structure):
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
                 ("weight_decay", ctypes.c_double), ("lr_dev", ctypes.c_void_p), ("grad_mul", ctypes.c_void_p),
-                ("grad_div", ctypes.c_void_p), ("found_inf", ctypes.c_void_p), ("seed", ctypes.c_uint32),
-                ("maximize", ctypes.c_int32)]
+                ("grad_div", ctypes.c_void_p), ("found_inf", ctypes.c_void_p), ("norm_coef2", ctypes.c_void_p),
+                ("norm_scratch", ctypes.c_void_p), ("norm_scratch_bytes", ctypes.c_size_t), ("max_norm", ctypes.c_double),
+                ("seed", ctypes.c_uint32), ("maximize", ctypes.c_int32)]
 
 
 def build(force: bool = False, jobs: int = 4) -> str:

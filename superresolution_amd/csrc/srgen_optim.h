@@ -13,6 +13,7 @@ namespace srgen {
 constexpr int kOptBlock = 32;        // elements that share one power-of-two scale (8-bit moments)
 constexpr int kOptChunk = 4096;      // elements of one workgroup of the step, and of one step counter
 constexpr int kOptMaxTensors = 240;  // tensors of one launch
+constexpr uint32_t kOptWavePartials = 1024;  // partial sums that one wave adds (in the step's own workgroups: no launch between)
 constexpr uint64_t kAddrMask = (1ull << 48) - 1;
 
 // One chunk of a list that takes steps (the table is made once for a list: it depends on the sizes alone).
@@ -29,6 +30,10 @@ struct AdamWScalars {
     const float* grad_mul;
     const float* grad_div;
     const float* found_inf;
+    const double* partial; // partial sums of the gradients' squares, or NULL: the step clips by their norm
+    double max_norm;
+    float* norm_coef;      // {norm, coefficient}, written by the first workgroup where partial is set
+    uint32_t partials;     // 1 .. kOptWavePartials
     uint32_t seed_key;     // mix(seed)
     int negate;
 };

@@ -24,9 +24,14 @@ namespace {
 // workgroups of 256 threads in one launch: the grid is counted in threads, in 32 bits
 constexpr uint64_t kMaxBlocks = (1ull << 24) - 1;
 
-// A step that moves more than this past the 256 MB Infinity Cache finds nothing of it there at the next step: its loads and stores
-// are marked non-temporal.
-constexpr uint64_t kStreamingBytes = 256ull << 20;
+// What a step touches (parameters, gradients, moments) is still in the 256 MB Infinity Cache at the next one, or was written by the
+// backward pass just now, unless it is larger than that: then loads and stores are marked non-temporal.  Measured, us without |
+// with: 32 bits fp32 20M parameters (320 MB) 93 | 105, 24M (384 MB) 135 | 126; bf16 24M (288 MB) 84 | 98, 32M (384 MB) 140 | 129;
+// 8 bits fp32 32M (322 MB) 87 | 91, 48M (483 MB) 151 | 135.
+constexpr uint64_t kStreamingBytes = 350ull << 20;
+// The norm only reads: 64 MB 14.4 | 12.7, 128 MB 24.4 | 22.8, 400 MB 74 | 65; but a step behind it finds small gradients in cache
+// (3M parameters with clipping 24 | 27).
+constexpr uint64_t kStreamingNormBytes = 128ull << 20;
 
 inline size_t element_bytes(int dtype) { return dtype == SRGEN_F32 ? 4 : 2; }
 inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
@@ -59,6 +64,42 @@ uint32_t norm_per_block(int count, const uint64_t* numel)
     uint64_t per = kOptChunk;
     while (per < (1u << 20) && total / per > 8192) per *= 2;
     return (uint32_t)per;
+}
+
+// the partial sums of the list's squares (tensors with g[i] == NULL are left out); the list has been checked
+int norm_partials(int count, const void* const* g, const uint64_t* numel, const int32_t* dtype, const float* norm_coef2, void* scratch,
+                  size_t scratch_bytes, void* stream, uint32_t* partials)
+{
+    if (!norm_coef2 || !aligned(norm_coef2, 4)) return fail(SRGEN_E_INVALID, "norm_coef2 is NULL or misaligned");
+    const uint32_t per = norm_per_block(count, numel);
+    uint64_t total = 0, bytes = 0;
+    for (int i = 0; i < count; ++i) {
+        if (!g[i]) continue;
+        total += chunks_of(numel[i], per);
+        bytes += numel[i] * element_bytes(dtype[i]);
+    }
+    if (total > 0xFFFFFFFFull) return fail(SRGEN_E_UNSUPPORTED, "%llu partial sums", (unsigned long long)total);
+    if (total && (!scratch || !aligned(scratch, 8))) return fail(SRGEN_E_INVALID, "scratch is NULL or misaligned");
+    if (scratch_bytes < total * sizeof(double))
+        return fail(SRGEN_E_WORKSPACE, "scratch of %zu bytes, %zu needed", scratch_bytes, (size_t)total * sizeof(double));
+    OptTensors ts;
+    uint64_t done = 0;
+    for (int i = 0; i < count;) {
+        uint64_t blocks = 0;
+        ts.count = 0;
+        for (; i < count && ts.count < kOptMaxTensors; ++i) {
+            const uint64_t c = g[i] ? chunks_of(numel[i], per) : 0;
+            if (blocks + c > kMaxBlocks) break;
+            if (!c) continue;
+            ts.t[ts.count++] = list_entry(g[i], numel[i], dtype[i], blocks);
+            blocks += c;
+        }
+        ts.partial0 = (uint32_t)done;
+        done += blocks;
+        if (blocks) HIP_TRY(launch_norm_partial(ts, bytes > kStreamingNormBytes, (uint32_t)blocks, per, (double*)scratch, (hipStream_t)stream));
+    }
+    *partials = (uint32_t)total;
+    return SRGEN_OK;
 }
 
 }  // namespace
@@ -106,7 +147,7 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
         return fail(SRGEN_E_INVALID, "lr %g, betas %g %g, eps %g, weight decay %g", args->lr, args->beta1, args->beta2, args->eps, args->weight_decay);
     uint64_t chunks = 0, step_bytes = 0;
     for (int i = 0; i < count; ++i) {
-        if (g[i]) step_bytes += numel[i] * (2 * element_bytes(p_dtype[i]) + element_bytes(g_dtype[i]) + (mo->bits == 32 ? 16 : 4));
+        if (g[i]) step_bytes += numel[i] * (element_bytes(p_dtype[i]) + element_bytes(g_dtype[i]) + (mo->bits == 32 ? 8 : 2));
         if (numel[i] && !p[i]) return fail(SRGEN_E_INVALID, "parameter %d is NULL", i);
         if (offset[i] % kOptBlock || offset[i] / kOptBlock > 0xFFFFFFFFull) return fail(SRGEN_E_INVALID, "offset %d: %llu", i, (unsigned long long)offset[i]);
         if (offset[i] + chunks_of(numel[i], kOptBlock) * kOptBlock > mo->numel)
@@ -119,9 +160,23 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
     if (!mo->m || !mo->v || !mo->step || !mo->table || (mo->bits == 8 && (!mo->m_scale || !mo->v_scale))) return fail(SRGEN_E_INVALID, "NULL moments");
     if (!aligned(mo->m, al) || !aligned(mo->v, al) || !aligned(mo->step, 4) || !aligned(mo->table, 16)) return fail(SRGEN_E_INVALID, "misaligned moments");
 
+    const float* mul = args->grad_mul;
+    const double* partial = nullptr;
+    uint32_t partials = 0;
+    if (args->norm_coef2) {
+        if (mul) return fail(SRGEN_E_INVALID, "grad_mul and norm_coef2: one of the two");
+        if (!(args->max_norm > 0.0)) return fail(SRGEN_E_INVALID, "max_norm %g", args->max_norm);
+        if (int rc = norm_partials(count, g, numel, g_dtype, args->norm_coef2, args->norm_scratch, args->norm_scratch_bytes, stream, &partials)) return rc;
+        if (partials && partials <= kOptWavePartials) partial = (const double*)args->norm_scratch;
+        else {
+            HIP_TRY(launch_norm_final((const double*)args->norm_scratch, partials, args->max_norm, args->norm_coef2, (hipStream_t)stream));
+            mul = args->norm_coef2 + 1;
+        }
+    }
     AdamWArgs a;
-    a.sc = AdamWScalars{args->beta1, args->beta2, log(args->beta1), log(args->beta2), args->lr, args->eps, args->weight_decay,
-                        args->lr_dev, args->grad_mul, args->grad_div, args->found_inf, opt_mix(args->seed), args->maximize};
+    a.sc = AdamWScalars{args->beta1, args->beta2, log(args->beta1), log(args->beta2), args->lr, args->eps, args->weight_decay, args->lr_dev,
+                        mul, args->grad_div, args->found_inf, partial, args->max_norm, args->norm_coef2, partials, opt_mix(args->seed),
+                        args->maximize};
     a.mo = MomentPtrs{mo->m, mo->v, mo->m_scale, mo->v_scale, mo->step, reinterpret_cast<const OptChunk*>(mo->table)};
     const bool streaming = step_bytes > kStreamingBytes;
     uint64_t done = 0;                                     // chunks of the launches so far
@@ -159,35 +214,9 @@ int srgen_total_norm(int count, const void* const* g, const uint64_t* numel, con
                      void* scratch, size_t scratch_bytes, void* stream)
 {
     if (int rc = check_list(count, g, numel, dtype, "tensor", true)) return rc;
-    if (!norm_coef2) return fail(SRGEN_E_INVALID, "norm_coef2 is NULL");
-    const uint32_t per = norm_per_block(count, numel);
-    uint64_t total = 0, bytes = 0;
-    for (int i = 0; i < count; ++i) {
-        if (!g[i]) continue;
-        total += chunks_of(numel[i], per);
-        bytes += numel[i] * element_bytes(dtype[i]);
-    }
-    if (total > 0xFFFFFFFFull) return fail(SRGEN_E_UNSUPPORTED, "%llu partial sums", (unsigned long long)total);
-    if (total && (!scratch || !aligned(scratch, 8))) return fail(SRGEN_E_INVALID, "scratch is NULL or misaligned");
-    if (scratch_bytes < total * sizeof(double))
-        return fail(SRGEN_E_WORKSPACE, "scratch of %zu bytes, %zu needed", scratch_bytes, (size_t)total * sizeof(double));
-    OptTensors ts;
-    uint64_t done = 0;
-    for (int i = 0; i < count;) {
-        uint64_t blocks = 0;
-        ts.count = 0;
-        for (; i < count && ts.count < kOptMaxTensors; ++i) {
-            const uint64_t c = g[i] ? chunks_of(numel[i], per) : 0;
-            if (blocks + c > kMaxBlocks) break;
-            if (!c) continue;
-            ts.t[ts.count++] = list_entry(g[i], numel[i], dtype[i], blocks);
-            blocks += c;
-        }
-        ts.partial0 = (uint32_t)done;
-        done += blocks;
-        if (blocks) HIP_TRY(launch_norm_partial(ts, bytes > kStreamingBytes, (uint32_t)blocks, per, (double*)scratch, (hipStream_t)stream));
-    }
-    HIP_TRY(launch_norm_final((const double*)scratch, (uint32_t)total, max_norm, norm_coef2, (hipStream_t)stream));
+    uint32_t partials = 0;
+    if (int rc = norm_partials(count, g, numel, dtype, norm_coef2, scratch, scratch_bytes, stream, &partials)) return rc;
+    HIP_TRY(launch_norm_final((const double*)scratch, partials, max_norm, norm_coef2, (hipStream_t)stream));
     return SRGEN_OK;
 }
 

@@ -284,6 +284,38 @@ __device__ inline bool roots(const float (&v)[V], float (&r)[V])
     return plain;
 }
 
+// ---- norm and clip coefficient from partial sums -----------------------------------------------------------------------
+__device__ inline double wave_sum(double x)
+{
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// the sum of up to kOptWavePartials numbers by one wave, in a fixed order; all its loads are requested at once
+__device__ inline double wave_total(const double* __restrict__ partial, uint32_t n)
+{
+    constexpr int U = kOptWavePartials / 64;
+    const uint32_t lane = threadIdx.x & 63;
+    double x[U], acc = 0.0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = lane + 64 * u < n ? partial[lane + 64 * u] : 0.0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc += x[u];
+    return wave_sum(acc);
+}
+
+// {sqrt(sum), min(1, max_norm / (norm + 1e-6))}; a NaN norm gives a NaN coefficient
+struct NormCoef {
+    float norm, coef;
+};
+__device__ inline NormCoef norm_coef_of(double sum, double max_norm)
+{
+    const float norm = (float)sqrt(sum);
+    const double c = max_norm / ((double)norm + 1e-6);
+    return NormCoef{norm, c > 1.0 ? 1.f : (float)c};
+}
+
 // ---- AdamW -------------------------------------------------------------------------------------------------------------
 //   g' = c g      m = b1 m + (1 - b1) g'      v = b2 v + (1 - b2) g'^2
 //   p  = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
@@ -436,6 +468,14 @@ __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScala
         const double bc1 = -expm1((double)t * sc.ln_beta1), bc2 = -expm1((double)t * sc.ln_beta2);
         const double s = lr / bc1;
         double f = sc.grad_mul ? (double)*sc.grad_mul : 1.0;
+        if (sc.partial) {
+            const NormCoef r = norm_coef_of(wave_total(sc.partial, sc.partials), sc.max_norm);
+            f = (double)r.coef;
+            if (tid == 0 && blockIdx.x == 0) {                         // (each launch's first: the same values)
+                sc.norm_coef[0] = r.norm;
+                sc.norm_coef[1] = r.coef;
+            }
+        }
         if (sc.grad_div) f /= (double)*sc.grad_div;
         if (sc.negate) f = -f;
         if (tid == 0) {
@@ -517,13 +557,6 @@ __device__ inline Found find_tensor(const OptTensors& ts, uint32_t blk)
 }
 
 // ---- total norm --------------------------------------------------------------------------------------------------------
-__device__ inline double wave_sum(double x)
-{
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d);
-    return x;
-}
-
 // 16 bytes of a list's tensor as 64-bit squares' sum; any alignment of the element
 template <int DT>
 struct Vec16 {
@@ -599,11 +632,19 @@ __global__ __launch_bounds__(256) void norm_partial_kernel(const OptTensors ts, 
     if (threadIdx.x == 0) partial[(size_t)ts.partial0 + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// norm_coef[0] = sqrt(sum), norm_coef[1] = min(1, max_norm / (norm + 1e-6)); a NaN norm gives a NaN coefficient
 __global__ __launch_bounds__(1024) void norm_final_kernel(const double* __restrict__ partial, uint32_t n, double max_norm,
                                                           float* __restrict__ norm_coef)
 {
     __shared__ double red[16];
+    if (n <= kOptWavePartials) {                             // (the order in which a step adds them)
+        if (threadIdx.x >= 64) return;
+        const NormCoef r = norm_coef_of(wave_total(partial, n), max_norm);
+        if (threadIdx.x == 0) {
+            norm_coef[0] = r.norm;
+            norm_coef[1] = r.coef;
+        }
+        return;
+    }
     double acc = 0.0;
     for (uint32_t i = threadIdx.x; i < n; i += 1024) acc += partial[i];
     acc = wave_sum(acc);
@@ -613,10 +654,9 @@ __global__ __launch_bounds__(1024) void norm_final_kernel(const double* __restri
         double s = 0.0;
 #pragma unroll
         for (int k = 0; k < 16; ++k) s += red[k];
-        const float norm = (float)sqrt(s);
-        const double c = max_norm / ((double)norm + 1e-6);
-        norm_coef[0] = norm;
-        norm_coef[1] = c > 1.0 ? 1.f : (float)c;
+        const NormCoef r = norm_coef_of(s, max_norm);
+        norm_coef[0] = r.norm;
+        norm_coef[1] = r.coef;
     }
 }
 
@@ -708,7 +748,7 @@ hipError_t launch_norm_partial(const OptTensors& ts, bool streaming, uint32_t bl
 
 hipError_t launch_norm_final(const double* partial, uint32_t n, double max_norm, float* norm_coef, hipStream_t s)
 {
-    hipLaunchKernelGGL(norm_final_kernel, dim3(1), dim3(1024), 0, s, partial, n, max_norm, norm_coef);
+    hipLaunchKernelGGL(norm_final_kernel, dim3(1), dim3(n <= kOptWavePartials ? 64 : 1024), 0, s, partial, n, max_norm, norm_coef);
     return hipGetLastError();
 }
 

@@ -126,6 +126,9 @@ class Moments:
         table = torch.empty((chunks, 4), dtype=torch.int32)                    # which chunk is where: of the sizes alone
         _lib.check(_lib.lib().srgen_adamw_chunk_table(len(self.numels), _addr(self._numel), _addr(self._offset), table.data_ptr(), chunks))
         self._table = table.to(device)
+        need = ctypes.c_size_t()
+        _lib.check(_lib.lib().srgen_total_norm_scratch_bytes(len(self.numels), self._sizes[0], need))
+        self.norm_bytes = need.value
         self._c = _lib.srgen_moments(bits, 0, *ptrs, self.step.data_ptr(), self._table.data_ptr(), self.total, chunks)
 
     @property
@@ -352,8 +355,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits={state_bits}: 8 or 32")
         if max_grad_norm is not None and not max_grad_norm > 0.0:
             raise ValueError(f"max_grad_norm={max_grad_norm}: positive, or None")
-        self.state_bits, self.max_grad_norm, self.seed = state_bits, max_grad_norm, int(seed) & 0xFFFFFFFF
-        self.last_grad_norm: Optional[torch.Tensor] = None
+        self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFF
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self._norm_coef: Optional[torch.Tensor] = None     # ends with {norm, clip coefficient} of the last step
         self.moments: List[Moments] = []
         self._lists: List[_Lists] = []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
@@ -378,6 +382,11 @@ class AdamW(torch.optim.Optimizer):
         # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
         self.moments.append(Moments([p.numel() for p in g["params"]], self.state_bits, dev))
         self._lists.append(_Lists(len(g["params"])))
+
+    @property
+    def last_grad_norm(self) -> Optional[torch.Tensor]:
+        """The gradients' total norm at the last step that clipped, before clipping (0-dim device tensor)."""
+        return None if self._norm_coef is None else self._norm_coef[-2]
 
     # -- one step -----------------------------------------------------------------------------------------------------
     def step(self, closure=None):
@@ -406,24 +415,27 @@ class AdamW(torch.optim.Optimizer):
         if not any(counts):
             return loss
         dev = self.moments[0].device
-        norm_coef = None
+        div, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        for t in (div, found):
+            if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != 1):
+                raise RuntimeError(f"AdamW: grad_scale and found_inf are fp32 scalars on {dev}")
+        mul = out = scratch = None
         if self.max_grad_norm is not None:
-            if len(counts) == 1:
-                ls = self._lists[0]
-                g, numel, code = ls.g, self.moments[0]._numel, ls.g_code
+            if div is not None:
+                raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
+                                   "scaler.step(optimizer)")
+            if len(counts) == 1:                           # norm and step in one call
+                mo = self.moments[0]
+                buf = torch.empty(mo.norm_bytes // 4 + 2, dtype=torch.float32, device=dev)
+                scratch = buf.data_ptr()
+                out = scratch + mo.norm_bytes
+                self._norm_coef = buf
             else:
                 g, numel, code = array("Q"), array("Q"), array("i")
                 for mo, ls in zip(self.moments, self._lists):
                     g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
-            norm_coef = _norm_coef(dev, g, numel, code, float(self.max_grad_norm))
-            self.last_grad_norm = norm_coef[0]
-        div, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
-        if norm_coef is not None and div is not None:
-            raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
-                               "scaler.step(optimizer)")
-        for t in (div, found):
-            if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != 1):
-                raise RuntimeError(f"AdamW: grad_scale and found_inf are fp32 scalars on {dev}")
+                self._norm_coef = _norm_coef(dev, g, numel, code, self.max_grad_norm)
+                mul = self._norm_coef.data_ptr() + 4
         with _on(dev):
             stream = _stream(dev)
             for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
@@ -438,9 +450,9 @@ class AdamW(torch.optim.Optimizer):
                         lr_dev, lr = lr.data_ptr(), 0.0
                     else:
                         lr = float(lr)
-                args = _lib.srgen_adamw_args(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev,
-                                             None if norm_coef is None else norm_coef.data_ptr() + 4, None if div is None else div.data_ptr(),
-                                             None if found is None else found.data_ptr(), self.seed, 1 if group["maximize"] else 0)
+                args = _lib.srgen_adamw_args(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, mul, None if div is None else div.data_ptr(),
+                                             None if found is None else found.data_ptr(), out, scratch, mo.norm_bytes,
+                                             self.max_grad_norm or 0.0, self.seed, 1 if group["maximize"] else 0)
                 mo._update(ls.pg, ls.codes, args, stream)
                 # the kernel wrote behind torch's back: the version counters are what the Generator / Discriminator mirrors
                 # watch to upload their weights again

@@ -124,7 +124,7 @@ def test_adamw_mixed_types(bits, pdt, gdt):
     (_, views), (_, gviews) = _make(sizes, DT[pdt], DT[gdt], seed=3)
     mo = optim.Moments(sizes, bits, torch.device("cuda", 0))
     refs = [R.AdamWRef(_f64(v), bits=bits, lr=1e-2, eps=1e-6, wd=0.0, offset=o, bf16=pdt == "bf16") for v, o in zip(views, mo.offsets)]
-    args = _lib.srgen_adamw_args(1e-2, 0.9, 0.999, 1e-6, 0.0, None, None, None, None, 0, 0)
+    args = _lib.srgen_adamw_args(1e-2, 0.9, 0.999, 1e-6, 0.0)
     code = {"fp32": 0, "bf16": 1}
     mo.update(array("Q", [v.data_ptr() for v in views]), array("Q", [v.data_ptr() for v in gviews]), array("i", [code[pdt]] * 2),
               array("i", [code[gdt]] * 2), args, torch.cuda.current_stream().cuda_stream)

@@ -19,7 +19,7 @@ def _adamw(numel=(64,), offset=(0,), p=(4096,), g=(8192,), pd=(0,), gd=(0,), cou
     """srgen_adamw_many with addresses that are never followed: every call here is refused before anything is launched."""
     L = _lib()
     mo = L.srgen_moments(32, 0, 1 << 20, 1 << 21, None, None, 1 << 22, 1 << 23, 64, 1)
-    args = L.srgen_adamw_args(1e-3, 0.9, 0.999, 1e-8, 0.0, None, None, None, None, 0, 0)
+    args = L.srgen_adamw_args(1e-3, 0.9, 0.999, 1e-8, 0.0)
     for k, v in over.items():
         setattr(mo if hasattr(mo, k) else args, k, v)
     a = [array("Q", p), array("Q", g), array("Q", numel), array("Q", offset), array("i", pd), array("i", gd)]
@@ -56,6 +56,11 @@ def _adamw(numel=(64,), offset=(0,), p=(4096,), g=(8192,), pd=(0,), gd=(0,), cou
     (dict(beta2=-0.1), -1, "betas"),
     (dict(eps=-1.0), -1, "eps"),
     (dict(weight_decay=float("nan")), -1, "weight decay"),
+    (dict(norm_coef2=64, max_norm=0.0), -1, "max_norm"),
+    (dict(norm_coef2=64, max_norm=1.0, grad_mul=64), -1, "one of the two"),
+    (dict(norm_coef2=66, max_norm=1.0), -1, "norm_coef2"),
+    (dict(norm_coef2=64, max_norm=1.0), -1, "scratch"),
+    (dict(norm_coef2=64, max_norm=1.0, norm_scratch=256, norm_scratch_bytes=4), -5, "scratch"),
 ])
 def test_adamw_many_refuses(kw, rc, text):
     got, msg = _adamw(**kw)
