@@ -544,15 +544,19 @@ struct Found {
     int dt;
     uint32_t block;         // in the tensor
 };
+// (every wave counts the tensors that start at or before the workgroup: four loads at once instead of eight one after another)
 __device__ inline Found find_tensor(const OptTensors& ts, uint32_t blk)
 {
-    int lo = 0, hi = ts.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (ts.t[mid].block0 <= blk) lo = mid;
-        else hi = mid - 1;
+    static_assert(kOptMaxTensors <= 256, "four entries a lane");
+    const int lane = threadIdx.x & 63;
+    int at = -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int k = lane + 64 * u;
+        const uint32_t first = ts.t[k < kOptMaxTensors ? k : 0].block0;
+        at += __popcll(__ballot(k < ts.count && first <= blk));
     }
-    const OptTensor& t = ts.t[lo];
+    const OptTensor& t = ts.t[__builtin_amdgcn_readfirstlane(at)];
     return Found{(const char*)(t.ptr & kAddrMask), t.numel_lo | (t.ptr >> 52) << 32, (int)(t.ptr >> 48) & 15, blk - t.block0};
 }
 
