@@ -247,12 +247,13 @@ class GanStep:
 
     def __init__(self, generator, discriminator, lr_g: float = 1e-4, lr_d: float = 1e-6, weight_adversarial: float = 0.005,
                  weight_pixel: float = 1.0, weight_ssim: float = 0.3, grad_clip_norm: float = 10.0, real_label: float = 0.9,
-                 fake_label: float = 0.1, group=None, precision: str = "auto", reuse_forward: bool = False):
+                 fake_label: float = 0.1, group=None, precision: str = "auto", reuse_forward: bool = False, state_bits: int = 32):
         # precision: the arithmetic of the generator's step, as PretrainStep ("auto": that of the autocast dtype, the way
         # train.py:148-149,166-167 call the generator); with "bf16" the discriminator's 64..512-channel convs take bf16
         # products too (DiscriminatorGrad.products), otherwise they stay on the exact-fp32 MFMA
         self.gen = PretrainStep(generator, lr=lr_g, ssim_weight=weight_ssim, l1_weight=weight_pixel, group=group,
-                                precision=precision)
+                                precision=precision, state_bits=state_bits)
+        # state_bits: of both optimizers' moments (8: optim.Moments)
         # reuse_forward: in an iteration that updates the discriminator the reference runs the generator twice on the same
         # batch (train.py:148-149 without a graph, :166-167 with one) and the generator's weights do not change in
         # between, so both calls return the same tensors bit for bit; ``step`` then keeps the first call's output and saved
@@ -263,7 +264,7 @@ class GanStep:
         self.opt_g = self.gen.optimizer
         self.ws = self.gen.ws
         self.d = discriminator
-        self.opt_d = FlatAdamW(discriminator.parameters(), lr=lr_d)
+        self.opt_d = FlatAdamW(discriminator.parameters(), lr=lr_d, state_bits=state_bits)
         self.dgrad = DiscriminatorGrad(discriminator, self.ws)
         self.w_adv, self.w_pix, self.w_ssim = weight_adversarial, weight_pixel, weight_ssim
         self.clip, self.real_label, self.fake_label, self.group = grad_clip_norm, real_label, fake_label, group

@@ -28,11 +28,23 @@ from torch.optim import optimizer as _torch_optimizer
 
 from . import _lib
 
+
+
+class _NotBuilt:
+    """Stands for an extension that is missing (the package can be imported to build it): raises where it is used."""
+
+    def __init__(self, why: Exception):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise _lib.SrgenError(f"{os.path.join(os.path.dirname(_lib.CSRC), '_tensorlist.so')} is missing or does not fit the installed "
+                              f"torch ({self._why}): run `python -c 'import __graft_entry__ as g; g.build()'`. There is no fallback path.")
+
+
 try:
     from . import _tensorlist
 except ImportError as e:
-    raise _lib.SrgenError(f"{os.path.join(os.path.dirname(_lib.CSRC), '_tensorlist.so')} is missing or does not fit the installed torch "
-                          f"({e}): run `python -c 'import __graft_entry__ as g; g.build()'`. There is no fallback path.") from e
+    _tensorlist = _NotBuilt(e)
 
 BLOCK = 32            # SRGEN_OPT_BLOCK: elements that share one scale (8-bit moments)
 CHUNK = 4096          # SRGEN_OPT_CHUNK: elements of one step counter
@@ -246,7 +258,7 @@ def _listed(tensors: List[torch.Tensor], what: str):
 
 
 def _norm_coef(dev: torch.device, ptr: array, numel: array, code: array, max_norm: float) -> torch.Tensor:
-    """Device floats {norm, clip coefficient}; address 0: left out."""
+    """A device buffer that ends with {norm, clip coefficient}; address 0: left out."""
     L, need = _lib.lib(), ctypes.c_size_t()
     _lib.check(L.srgen_total_norm_scratch_bytes(len(ptr), _addr(numel), need))
     words = need.value // 4
@@ -254,7 +266,7 @@ def _norm_coef(dev: torch.device, ptr: array, numel: array, code: array, max_nor
     with _on(dev):
         _lib.check(L.srgen_total_norm(len(ptr), _addr(ptr), _addr(numel), _addr(code), max_norm, buf.data_ptr() + need.value, buf.data_ptr(),
                                       need.value, _stream(dev)))
-    return buf[words:]
+    return buf
 
 
 def total_norm(tensors) -> torch.Tensor:
@@ -265,7 +277,7 @@ def total_norm(tensors) -> torch.Tensor:
     if not ts:
         return torch.tensor(0.0)
     dev, ts, ptr, numel, code = _listed(ts, "total_norm")
-    return _norm_coef(dev, ptr, numel, code, 1.0)[0]
+    return _norm_coef(dev, ptr, numel, code, 1.0)[-2]
 
 
 def _grads(parameters) -> List[torch.Tensor]:
@@ -294,7 +306,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
         if g is not t:
             raise RuntimeError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or overlaps")
     _no_overlap([(a, n * (4 if c == _lib.SRGEN_F32 else 2)) for a, n, c in zip(ptr, numel, code)], "clip_grad_norm_")
-    out = _norm_coef(dev, ptr, numel, code, float(max_norm))
+    out = _norm_coef(dev, ptr, numel, code, float(max_norm))[-2:]
     if error_if_nonfinite and not bool(torch.isfinite(out[0])):
         raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To "
                            "disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
@@ -435,7 +447,7 @@ class AdamW(torch.optim.Optimizer):
                 for mo, ls in zip(self.moments, self._lists):
                     g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
                 self._norm_coef = _norm_coef(dev, g, numel, code, self.max_grad_norm)
-                mul = self._norm_coef.data_ptr() + 4
+                mul = self._norm_coef.data_ptr() + 4 * (self._norm_coef.numel() - 1)
         with _on(dev):
             stream = _stream(dev)
             for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):

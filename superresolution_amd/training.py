@@ -14,11 +14,13 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+from array import array
 from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import _lib
+from .optim import Moments
 
 WINO_FLOATS = 16 * 96 * 96           # Winograd weight image of one 96 -> 96 conv
 SPLIT_HALFS = 2 * 9 * 96 * 96         # split-f16 weight image of one 96 -> 96 conv: (hi, lo) per weight
@@ -518,9 +520,13 @@ class FlatAdamW(torch.optim.Optimizer):
     buffer: the parameters are re-pointed at views of it, so one kernel launch updates every tensor and the data-parallel
     gradient all-reduce of the training configurations is one collective over ``flat_grad`` (12.86 MB for the generator).
     A ``torch.optim.Optimizer`` with one parameter group, so the reference's ``ReduceLROnPlateau`` (train.py:76-79) and
-    ``optimizer.param_groups[0]['lr']`` (train.py:106) work on it unchanged; ``state_dict`` holds the flat moments."""
+    ``optimizer.param_groups[0]['lr']`` (train.py:106) work on it unchanged; ``state_dict`` holds the flat moments.
+    ``state_bits=8`` holds both moments in 8 bits (``optim.Moments``: a quarter of the memory and of the traffic)."""
 
-    def __init__(self, params, lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01):
+    def __init__(self, params, lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 state_bits: int = 32, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits={state_bits}: 8 or 32")
         plist = [p for p in params]
         if not plist or not all(p.is_cuda and p.dtype == torch.float32 for p in plist):
             raise RuntimeError("FlatAdamW needs fp32 parameters on a ROCm device; there is no CPU fallback")
@@ -530,7 +536,11 @@ class FlatAdamW(torch.optim.Optimizer):
         n = sum(p.numel() for p in plist)
         self.flat = torch.empty(n, dtype=torch.float32, device=dev)
         self.flat_grad = torch.zeros(n, dtype=torch.float32, device=dev)
-        self.exp_avg, self.exp_avg_sq = torch.zeros_like(self.flat), torch.zeros_like(self.flat)
+        self.moments, self.seed = None, int(seed) & 0xFFFFFFFF
+        if state_bits == 8:
+            self.moments = Moments([n], 8, dev)
+        else:
+            self.exp_avg, self.exp_avg_sq = torch.zeros_like(self.flat), torch.zeros_like(self.flat)
         off = 0
         self._grad_views = []
         with torch.no_grad():
@@ -552,6 +562,15 @@ class FlatAdamW(torch.optim.Optimizer):
             raise NotImplementedError("FlatAdamW.step takes no closure")
         g = self.param_groups[0]
         self.steps += 1
+        if self.moments is not None:
+            with torch.cuda.device(self.flat.device):
+                args = _lib.srgen_adamw_args(float(g["lr"]), *map(float, g["betas"]), float(g["eps"]), float(g["weight_decay"]),
+                                             seed=self.seed)
+                fp32 = array("i", [_lib.SRGEN_F32])
+                self.moments.update(array("Q", [self.flat.data_ptr()]), array("Q", [self.flat_grad.data_ptr()]), fp32, fp32, args,
+                                    _stream(self.flat))
+            torch.autograd.graph.increment_version(self.params)
+            return
         with torch.cuda.device(self.flat.device):
             _lib.check(_lib.lib().srgen_adamw(self.flat.data_ptr(), self.flat_grad.data_ptr(), self.exp_avg.data_ptr(),
                                               self.exp_avg_sq.data_ptr(), self.flat.numel(), float(g["lr"]),
@@ -581,12 +600,13 @@ class FlatAdamW(torch.optim.Optimizer):
         g = {k: v for k, v in self.param_groups[0].items() if k != "params"}
         g["params"] = list(range(len(self.params)))
         state, off = {}, 0
-        if self.steps > 0:
+        steps = self.steps if self.moments is None else self.moments.steps()[0]      # (8 bits: counted on the device)
+        if steps > 0:
+            m, v = (self.exp_avg, self.exp_avg_sq) if self.moments is None else self.moments.read()
             for i, p in enumerate(self.params):
                 k = p.numel()
-                state[i] = {"step": torch.tensor(float(self.steps)),
-                            "exp_avg": self.exp_avg[off:off + k].view(p.shape).clone(),
-                            "exp_avg_sq": self.exp_avg_sq[off:off + k].view(p.shape).clone()}
+                state[i] = {"step": torch.tensor(float(steps)), "exp_avg": m[off:off + k].view(p.shape).clone(),
+                            "exp_avg_sq": v[off:off + k].view(p.shape).clone()}
                 off += k
         return {"state": state, "param_groups": [g]}
 
@@ -596,9 +616,10 @@ class FlatAdamW(torch.optim.Optimizer):
         if "state" not in sd:                                            # (the former private layout)
             if sd["exp_avg"].numel() != self.flat.numel():
                 raise ValueError(f"optimizer state has {sd['exp_avg'].numel()} entries, the parameters {self.flat.numel()}")
-            self.steps = int(sd["step"])
-            self.exp_avg.copy_(sd["exp_avg"])
-            self.exp_avg_sq.copy_(sd["exp_avg_sq"])
+            m, v = self._fp32_moments()
+            m[:self.flat.numel()].copy_(sd["exp_avg"])
+            v[:self.flat.numel()].copy_(sd["exp_avg_sq"])
+            self._take_moments(m, v, int(sd["step"]))
             self.param_groups[0].update({k: v for k, v in sd["param_groups"][0].items() if k != "params"})
             return
         groups = sd["param_groups"]
@@ -610,9 +631,9 @@ class FlatAdamW(torch.optim.Optimizer):
         steps = {int(float(st["step"])) for st in state.values()}
         if len(steps) > 1:
             raise ValueError(f"per-parameter step counts differ ({sorted(steps)}): one flat AdamW has one step count")
-        self.steps = steps.pop() if steps else 0
-        self.exp_avg.zero_()
-        self.exp_avg_sq.zero_()
+        m, v = self._fp32_moments()
+        m.zero_()
+        v.zero_()
         off = 0
         for i, p in zip(ids, self.params):
             k = p.numel()
@@ -620,10 +641,24 @@ class FlatAdamW(torch.optim.Optimizer):
             if st is not None:
                 if st["exp_avg"].numel() != k:
                     raise ValueError(f"optimizer state of parameter {i} has {st['exp_avg'].numel()} entries, the parameter {k}")
-                self.exp_avg[off:off + k].copy_(st["exp_avg"].reshape(-1))
-                self.exp_avg_sq[off:off + k].copy_(st["exp_avg_sq"].reshape(-1))
+                m[off:off + k].copy_(st["exp_avg"].reshape(-1))
+                v[off:off + k].copy_(st["exp_avg_sq"].reshape(-1))
             off += k
+        self._take_moments(m, v, steps.pop() if steps else 0)
         self.param_groups[0].update({k: v for k, v in groups[0].items() if k != "params"})
+
+    def _fp32_moments(self):
+        """fp32 buffers to load moments into: the moments themselves, or (8 bits) new ones that ``_take_moments`` packs."""
+        if self.moments is None:
+            return self.exp_avg, self.exp_avg_sq
+        m = torch.zeros(self.moments.total, dtype=torch.float32, device=self.flat.device)
+        return m, torch.zeros_like(m)
+
+    def _take_moments(self, m: torch.Tensor, v: torch.Tensor, steps: int) -> None:
+        self.steps = steps
+        if self.moments is not None:
+            self.moments.write(m, v)
+            self.moments.set_steps([steps])
 
 
 # ---- the residual block (Generator.py:30-42) in train mode: forward with saved tensors, backward ----------------------
@@ -1034,12 +1069,12 @@ class PretrainStep(GeneratorGrad):
     ranks with one all-reduce before the update, as DistributedDataParallel would."""
 
     def __init__(self, generator, lr: float = 1e-4, ssim_weight: float = 0.1, l1_weight: float = 1.0, group=None,
-                 precision: str = "auto"):
+                 precision: str = "auto", state_bits: int = 32):
         if precision not in ("auto", "fp32", "f16", "bf16"):
             raise RuntimeError(f"precision '{precision}': expected auto, fp32, f16 or bf16")
         self.precision = precision
         super().__init__(generator)
-        self.optimizer = FlatAdamW(generator.parameters(), lr=lr)
+        self.optimizer = FlatAdamW(generator.parameters(), lr=lr, state_bits=state_bits)     # (8: moments in 8 bits)
         self.ssim_weight, self.l1_weight, self.group = ssim_weight, l1_weight, group
         self.last_metrics = None
 

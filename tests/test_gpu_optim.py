@@ -765,3 +765,66 @@ def test_the_reference_loop_with_these_operators(bits):
         assert torch.isfinite(gen(lr_img)).all()                          # (the weights are uploaded again)
     sd = opt.state_dict()
     assert len(sd["state"]) == 167 and float(sd["state"][0]["step"]) == 2.0
+
+
+def test_flat_adamw_with_8_bit_moments():
+    """training.FlatAdamW(state_bits=8) is the list's step on its one flat buffer; its checkpoints are those of 32 bits."""
+    from superresolution_amd import optim
+    from superresolution_amd.training import FlatAdamW
+    sizes = [300, 1, 5000]
+    init = [_hash_floats(n, i).cuda() for i, n in enumerate(sizes)]
+    ps = [torch.nn.Parameter(x.clone()) for x in init]
+    a = FlatAdamW(ps, lr=1e-3, state_bits=8, seed=4)
+    one = torch.nn.Parameter(torch.cat(init))
+    b = optim.AdamW([one], lr=1e-3, weight_decay=0.01, state_bits=8, seed=4)
+    for s in range(3):
+        g = _hash_floats(sum(sizes), 20 + s, 1e-2).cuda()
+        a.zero_grad()
+        a.flat_grad.copy_(g)
+        one.grad = g.clone()
+        before = [p._version for p in ps]
+        a.step()
+        b.step()
+        assert all(p._version > v for p, v in zip(ps, before))
+    assert torch.equal(a.flat, one) and torch.equal(a.moments.exp_avg.view(torch.uint8), b.moments[0].exp_avg.view(torch.uint8))
+    sd = a.state_dict()
+    assert float(sd["state"][0]["step"]) == 3.0 and sd["state"][2]["exp_avg"].shape == (5000,)
+    c = FlatAdamW([torch.nn.Parameter(x.clone()) for x in init], lr=1.0, state_bits=8)
+    c.load_state_dict(sd)
+    assert c.steps == 3 and c.param_groups[0]["lr"] == 1e-3 and c.moments.steps() == [3]
+    assert all(torch.equal(x, y) for x, y in zip(a.moments.read(), c.moments.read()))
+    d = FlatAdamW([torch.nn.Parameter(x.clone()) for x in init], lr=1.0)          # 8 -> 32 bits -> torch
+    d.load_state_dict(sd)
+    assert torch.equal(d.exp_avg, a.moments.read()[0][:sum(sizes)])
+    torch.optim.AdamW([torch.nn.Parameter(x.clone()) for x in init], lr=1.0).load_state_dict(d.state_dict())
+    e = FlatAdamW([torch.nn.Parameter(x.clone()) for x in init], lr=1.0, state_bits=8)
+    e.load_state_dict({"step": 3, "exp_avg": d.exp_avg, "exp_avg_sq": d.exp_avg_sq, "param_groups": sd["param_groups"]})
+    assert all(torch.equal(x, y) for x, y in zip(a.moments.read(), e.moments.read()))
+
+
+def test_fused_training_steps_with_8_bit_moments():
+    """PretrainStep and GanStep with state_bits=8: the first step's gradients are those of 32 bits, the update's sizes are alike."""
+    from superresolution_amd import Discriminator, Generator
+    from superresolution_amd.gan_training import GanStep
+    from superresolution_amd.training import PretrainStep
+    lr_img, hr = torch.rand(2, 3, 64, 64, device="cuda"), torch.rand(2, 3, 125, 125, device="cuda")
+    flats = []
+    for bits in (32, 8):
+        torch.manual_seed(3)
+        gen = Generator().cuda().train()
+        step = PretrainStep(gen, lr=1e-4, state_bits=bits)
+        start = step.optimizer.flat.clone()
+        step.step(lr_img, hr)
+        flats.append((start, step.optimizer.flat_grad.clone(), step.optimizer.flat.clone()))
+    assert torch.equal(flats[0][1], flats[1][1])
+    # From zero moments m = (1 - b1) g and v = (1 - b2) g^2 before they are stored, so the first update is that of 32 bits but for
+    # fp32 roundings: 1 - b2 in FlatAdamW's kernel is a float's (5e-5 of it off), which is 3e-5 of an update of lr
+    moved = (flats[0][2] - flats[0][0]).abs().max()
+    assert float((flats[0][2] - flats[1][2]).abs().max()) <= 1e-4 * float(moved) + 2e-8
+    torch.manual_seed(3)
+    gan = GanStep(Generator().cuda().train(), Discriminator().cuda().train(), state_bits=8)
+    for _ in range(2):
+        out = gan.step(lr_img, hr)
+    assert all(torch.isfinite(v) for v in out.values()) and gan.opt_g.moments.steps() == [2] and gan.opt_d.moments.steps() == [2]
+    assert torch.isfinite(gan.opt_g.flat).all() and torch.isfinite(gan.opt_d.flat).all()
+    assert gan.opt_d.moments.nbytes < 0.27 * 8 * gan.opt_d.flat.numel()
