@@ -32,7 +32,7 @@ struct AdamWScalars {
     const float* found_inf;
     const double* partial; // partial sums of the gradients' squares, or NULL: the step clips by their norm
     double max_norm;
-    float* norm_coef;      // {norm, coefficient}, written by the first workgroup where partial is set
+    float* norm_coef;      // {norm, coefficient}, written where partial is set
     uint32_t partials;     // 1 .. kOptWavePartials
     uint32_t seed_key;     // mix(seed)
     int negate;

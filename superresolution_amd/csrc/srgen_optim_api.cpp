@@ -155,24 +155,27 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
         chunks += chunks_of(numel[i], kOptChunk);
     }
     if (chunks != mo->chunks) return fail(SRGEN_E_INVALID, "moments of %llu chunks, the list has %llu", (unsigned long long)mo->chunks, (unsigned long long)chunks);
-    if (!chunks) return SRGEN_OK;
+    if (args->norm_coef2) {
+        if (args->grad_mul) return fail(SRGEN_E_INVALID, "grad_mul and norm_coef2: one of the two");
+        if (!(args->max_norm > 0.0)) return fail(SRGEN_E_INVALID, "max_norm %g", args->max_norm);
+    }
     const size_t al = mo->bits == 32 ? 16 : 4;
-    if (!mo->m || !mo->v || !mo->step || !mo->table || (mo->bits == 8 && (!mo->m_scale || !mo->v_scale))) return fail(SRGEN_E_INVALID, "NULL moments");
+    if (chunks && (!mo->m || !mo->v || !mo->step || !mo->table || (mo->bits == 8 && (!mo->m_scale || !mo->v_scale)))) return fail(SRGEN_E_INVALID, "NULL moments");
     if (!aligned(mo->m, al) || !aligned(mo->v, al) || !aligned(mo->step, 4) || !aligned(mo->table, 16)) return fail(SRGEN_E_INVALID, "misaligned moments");
 
     const float* mul = args->grad_mul;
     const double* partial = nullptr;
     uint32_t partials = 0;
     if (args->norm_coef2) {
-        if (mul) return fail(SRGEN_E_INVALID, "grad_mul and norm_coef2: one of the two");
-        if (!(args->max_norm > 0.0)) return fail(SRGEN_E_INVALID, "max_norm %g", args->max_norm);
         if (int rc = norm_partials(count, g, numel, g_dtype, args->norm_coef2, args->norm_scratch, args->norm_scratch_bytes, stream, &partials)) return rc;
-        if (partials && partials <= kOptWavePartials) partial = (const double*)args->norm_scratch;
+        // (found_inf may end the step's workgroups before they add anything, and the norm is wanted all the same)
+        if (partials && partials <= kOptWavePartials && !args->found_inf) partial = (const double*)args->norm_scratch;
         else {
             HIP_TRY(launch_norm_final((const double*)args->norm_scratch, partials, args->max_norm, args->norm_coef2, (hipStream_t)stream));
             mul = args->norm_coef2 + 1;
         }
     }
+    if (!chunks) return SRGEN_OK;
     AdamWArgs a;
     a.sc = AdamWScalars{args->beta1, args->beta2, log(args->beta1), log(args->beta2), args->lr, args->eps, args->weight_decay, args->lr_dev,
                         mul, args->grad_div, args->found_inf, partial, args->max_norm, args->norm_coef2, partials, opt_mix(args->seed),

@@ -352,6 +352,7 @@ struct Chunk {
     uint8_t* ve;
     uint32_t n, np;                    // elements; the same in whole blocks of 32
     uint32_t lo, w;                    // position: its low word; that with the high word mixed in
+    bool first;                        // of its tensor
 };
 
 template <int BITS, int PDT, int GDT, int V, bool FULL, bool NT>
@@ -471,7 +472,7 @@ __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScala
         if (sc.partial) {
             const NormCoef r = norm_coef_of(wave_total(sc.partial, sc.partials), sc.max_norm);
             f = (double)r.coef;
-            if (tid == 0 && blockIdx.x == 0) {                         // (each launch's first: the same values)
+            if (tid == 0 && c.first) {                                 // (of every tensor that takes the step: the same values)
                 sc.norm_coef[0] = r.norm;
                 sc.norm_coef[1] = r.coef;
             }
@@ -527,7 +528,7 @@ __global__ __launch_bounds__(256) void adamw_many_kernel(const AdamWArgs a)
     const uint64_t base = (uint64_t)ck.index * kOptChunk, off = (uint64_t)ck.offset32 * kOptBlock;
     const Chunk c{(void*)((pw & kAddrMask) + base * (pdt ? 2 : 4)), (const void*)((gw & kAddrMask) + base * (gdt ? 2 : 4)),
                   (uint8_t*)a.mo.m + off * (BITS / 8), (uint8_t*)a.mo.v + off * (BITS / 8), a.mo.m_scale + ck.offset32, a.mo.v_scale + ck.offset32,
-                  ck.count, round_up_block(ck.count), (uint32_t)off, (uint32_t)off + (uint32_t)(off >> 32) * kGold};
+                  ck.count, round_up_block(ck.count), (uint32_t)off, (uint32_t)off + (uint32_t)(off >> 32) * kGold, ck.index == 0};
     if (pdt == 0) {
         if (gdt == 0) adamw_chunk_any<BITS, 0, 0, NT>(a, c, &shared);
         else adamw_chunk_any<BITS, 0, 1, NT>(a, c, &shared);

@@ -357,7 +357,11 @@ class AdamW(torch.optim.Optimizer):
     then follows it.  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
     optimizer have to stay.  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
     gradient does not happen.  ``state_dict`` has the layout of ``torch.optim.AdamW`` with fp32 moments, whatever
-    ``state_bits``: checkpoints move between the two, and between 8 and 32 bits."""
+    ``state_bits``: checkpoints move between the two, and between 8 and 32 bits.
+
+    The random bits do not depend on the process: data-parallel ranks that take the same gradients stay the same bit for bit.
+    A second moment beyond fp32's range (gradients of some 1e20) is infinite with 32 bits, which stops the element, and NaN with
+    8.  Steps of one optimizer must not overlap, neither on two streams nor from two threads."""
 
     _step_supports_amp_scaling = True
 

@@ -275,6 +275,44 @@ def test_clip_inside_the_step(bits, max_norm):
     assert all(torch.equal(a, b) for a, b in zip(keep, gviews))
 
 
+@pytest.mark.parametrize("sizes", [[5_000_003, 7], [100] * 1100, [0, 0]])
+def test_clip_inside_the_step_with_more_partial_sums_than_a_wave_adds(sizes):
+    """More than 1,024 partial sums take a launch of their own; a list of empty tensors has norm 0.  Against clipping in place."""
+    from superresolution_amd import optim
+    ps = [torch.nn.Parameter(_hash_floats(n, i).cuda()) for i, n in enumerate(sizes)]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    for i, (p, q) in enumerate(zip(ps, qs)):
+        p.grad = _hash_floats(p.numel(), 5000 + i, 1e-2).cuda()
+        q.grad = p.grad.clone()
+    a, b = optim.AdamW(ps, lr=1e-2, max_grad_norm=0.5), optim.AdamW(qs, lr=1e-2)
+    a.step()
+    norm = optim.clip_grad_norm_(qs, 0.5)
+    b.step()
+    assert torch.equal(a.last_grad_norm, norm) and all(torch.equal(p, q) for p, q in zip(ps, qs))
+    want = np.sqrt(sum((_f64(p.grad) ** 2).sum() for p in ps))
+    assert abs(float(norm) - want) <= 1.01 * R.U24 * want
+
+
+def test_clipping_norm_where_the_first_tensors_have_no_gradient_or_the_step_is_skipped():
+    from superresolution_amd import optim
+    ps = [torch.nn.Parameter(_hash_floats(50, i).cuda()) for i in range(300)]
+    for i in (7, 299):
+        ps[i].grad = _hash_floats(50, 70 + i).cuda()
+    want = optim.total_norm([ps[7].grad, ps[299].grad])
+    opt = optim.AdamW(ps, lr=1e-2, max_grad_norm=0.1)
+    assert opt.last_grad_norm is None
+    for _ in range(3):                                                  # (the buffer's earlier contents do not help)
+        torch.full((4096,), float("nan"), device="cuda")
+        opt.step()
+        assert torch.equal(opt.last_grad_norm, want)
+    keep = ps[7].detach().clone()
+    opt.found_inf = torch.ones((), device="cuda")
+    torch.full((4096,), float("nan"), device="cuda")
+    opt.step()
+    assert torch.equal(opt.last_grad_norm, want) and torch.equal(ps[7], keep)
+    assert opt.moments[0].steps()[7] == 3 and opt.moments[0].steps()[0] == 0
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_step_follows_the_learning_rate_and_counts(bits):
     """A captured step replayed five times, with eager work and synchronisation between, against eager steps; the learning
