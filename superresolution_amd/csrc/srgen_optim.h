@@ -70,7 +70,7 @@ static_assert(sizeof(OptTensors) <= 4096 - 64, "kernel arguments hold 4 KiB");
 
 uint32_t opt_mix(uint32_t x);        // the hash of the stochastic rounding (host side, for the seed)
 
-hipError_t launch_adamw_many(const AdamWArgs& a, int bits, bool streaming, uint32_t blocks, hipStream_t s);
+hipError_t launch_adamw_many(const AdamWArgs& a, int bits, int list, bool streaming, uint32_t blocks, hipStream_t s);
 hipError_t launch_norm_partial(const OptTensors& ts, bool streaming, uint32_t blocks, uint32_t per_block, double* partial, hipStream_t s);
 hipError_t launch_norm_final(const double* partial, uint32_t n, double max_norm, float* norm_coef, hipStream_t s);
 hipError_t launch_scale_many(const OptTensors& ts, uint32_t blocks, const float* coef, hipStream_t s);

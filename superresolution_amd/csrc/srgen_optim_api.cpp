@@ -146,7 +146,9 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
         !(args->beta2 >= 0.0 && args->beta2 < 1.0))
         return fail(SRGEN_E_INVALID, "lr %g, betas %g %g, eps %g, weight decay %g", args->lr, args->beta1, args->beta2, args->eps, args->weight_decay);
     uint64_t chunks = 0, step_bytes = 0;
+    unsigned types = 0;                                    // bit 0: some fp32, bit 1: some bf16
     for (int i = 0; i < count; ++i) {
+        if (g[i]) types |= 1u << p_dtype[i] | 1u << g_dtype[i];
         if (g[i]) step_bytes += numel[i] * (element_bytes(p_dtype[i]) + element_bytes(g_dtype[i]) + (mo->bits == 32 ? 8 : 2));
         if (numel[i] && !p[i]) return fail(SRGEN_E_INVALID, "parameter %d is NULL", i);
         if (offset[i] % kOptBlock || offset[i] / kOptBlock > 0xFFFFFFFFull) return fail(SRGEN_E_INVALID, "offset %d: %llu", i, (unsigned long long)offset[i]);
@@ -198,7 +200,7 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
         }
         a.chunk0 = (uint32_t)done;
         done += blocks;
-        if (any) HIP_TRY(launch_adamw_many(a, mo->bits, streaming, (uint32_t)blocks, (hipStream_t)stream));
+        if (any) HIP_TRY(launch_adamw_many(a, mo->bits, types == 1 ? 0 : types == 2 ? 1 : 2, streaming, (uint32_t)blocks, (hipStream_t)stream));
     }
     return SRGEN_OK;
 }

@@ -332,6 +332,19 @@ struct StepScalars {
     uint32_t key;
 };
 
+// (the same for the workgroup: in scalar registers)
+__device__ inline uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ inline float uniform(float x) { return __uint_as_float(uniform(__float_as_uint(x))); }
+__device__ inline double uniform(double x)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)uniform((uint32_t)b) | (uint64_t)uniform((uint32_t)(b >> 32)) << 32);
+}
+__device__ inline StepScalars uniform(const StepScalars& s)
+{
+    return StepScalars{uniform(s.c1), uniform(s.c2), uniform(s.decay), uniform(s.ra), uniform(s.rb), uniform(s.gmul), uniform(s.key)};
+}
+
 // what a thread reads for its V elements
 template <int BITS, int PDT, int GDT, int V>
 struct Operands {
@@ -453,10 +466,9 @@ __device__ inline void update(const AdamWScalars& sc, const StepScalars& sh, con
     }
 }
 
-template <int BITS, int PDT, int GDT, bool FULL, bool NT>
+template <int BITS, int PDT, int GDT, int V, bool FULL, bool NT>
 __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScalars* shared)
 {
-    constexpr int V = BITS == 8 && PDT == 1 && GDT == 1 ? 8 : 4;
     constexpr uint32_t STRIDE = 256 * V;
     const AdamWScalars& sc = a.sc;
     const uint32_t tid = threadIdx.x;
@@ -492,7 +504,7 @@ __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScala
         }
     }
     __syncthreads();
-    const StepScalars sh = *shared;
+    const StepScalars sh = uniform(*shared);
     if constexpr (FULL) {
 #pragma unroll 2
         for (uint32_t i0 = 0; i0 < kOptChunk; i0 += STRIDE) {
@@ -509,14 +521,17 @@ __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScala
     }
 }
 
-template <int BITS, int PDT, int GDT, bool NT>
+template <int BITS, int PDT, int GDT, int V, bool NT>
 __device__ inline void adamw_chunk_any(const AdamWArgs& a, const Chunk& c, StepScalars* shared)
 {
-    if (c.n == kOptChunk && c.lo + (kOptChunk - 1) >= c.lo) adamw_chunk<BITS, PDT, GDT, true, NT>(a, c, shared);
-    else adamw_chunk<BITS, PDT, GDT, false, NT>(a, c, shared);
+    if (c.n == kOptChunk && c.lo + (kOptChunk - 1) >= c.lo) adamw_chunk<BITS, PDT, GDT, V, true, NT>(a, c, shared);
+    else adamw_chunk<BITS, PDT, GDT, V, false, NT>(a, c, shared);
 }
 
-template <int BITS, bool NT>
+// LIST: types of the list's parameters and gradients: 0 all fp32, 1 all bf16, 2 mixed.  Kernels of their own for the first two leave
+// each the registers that its own path needs: 6 workgroups a CU instead of 4 for fp32 with 8 bits (discriminator's step 18.2 -> 17.5
+// us), 5 instead of 4 for bf16 (268M parameters 498 -> 484 us).
+template <int BITS, int LIST, bool NT>
 __global__ __launch_bounds__(256) void adamw_many_kernel(const AdamWArgs a)
 {
     __shared__ StepScalars shared;
@@ -524,17 +539,19 @@ __global__ __launch_bounds__(256) void adamw_many_kernel(const AdamWArgs a)
     const uint64_t pw = a.p[ck.tensor - a.tensor0], gw = a.g[ck.tensor - a.tensor0];
     if (gw == 0) return;
     if (a.sc.found_inf && *a.sc.found_inf != 0.f) return;
-    const int pdt = (int)(pw >> 48), gdt = (int)(gw >> 48);
+    const int pdt = LIST == 2 ? (int)(pw >> 48) : LIST, gdt = LIST == 2 ? (int)(gw >> 48) : LIST;
     const uint64_t base = (uint64_t)ck.index * kOptChunk, off = (uint64_t)ck.offset32 * kOptBlock;
     const Chunk c{(void*)((pw & kAddrMask) + base * (pdt ? 2 : 4)), (const void*)((gw & kAddrMask) + base * (gdt ? 2 : 4)),
                   (uint8_t*)a.mo.m + off * (BITS / 8), (uint8_t*)a.mo.v + off * (BITS / 8), a.mo.m_scale + ck.offset32, a.mo.v_scale + ck.offset32,
                   ck.count, round_up_block(ck.count), (uint32_t)off, (uint32_t)off + (uint32_t)(off >> 32) * kGold, ck.index == 0};
-    if (pdt == 0) {
-        if (gdt == 0) adamw_chunk_any<BITS, 0, 0, NT>(a, c, &shared);
-        else adamw_chunk_any<BITS, 0, 1, NT>(a, c, &shared);
+    if constexpr (LIST == 0) adamw_chunk_any<BITS, 0, 0, 4, NT>(a, c, &shared);
+    else if constexpr (LIST == 1) adamw_chunk_any<BITS, 1, 1, BITS == 8 ? 8 : 4, NT>(a, c, &shared);
+    else if (pdt == 0) {
+        if (gdt == 0) adamw_chunk_any<BITS, 0, 0, 4, NT>(a, c, &shared);
+        else adamw_chunk_any<BITS, 0, 1, 4, NT>(a, c, &shared);
     } else {
-        if (gdt == 0) adamw_chunk_any<BITS, 1, 0, NT>(a, c, &shared);
-        else adamw_chunk_any<BITS, 1, 1, NT>(a, c, &shared);
+        if (gdt == 0) adamw_chunk_any<BITS, 1, 0, 4, NT>(a, c, &shared);
+        else adamw_chunk_any<BITS, 1, 1, 4, NT>(a, c, &shared);
     }
 }
 
@@ -736,11 +753,24 @@ __global__ __launch_bounds__(256) void moments_unpack_kernel(const uint8_t* __re
 
 uint32_t opt_mix(uint32_t x) { return mix32(x); }
 
-hipError_t launch_adamw_many(const AdamWArgs& a, int bits, bool streaming, uint32_t blocks, hipStream_t s)
+template <int BITS>
+static void (*adamw_kernel_of(int list, bool streaming))(AdamWArgs)
 {
-    auto* k = bits == 32 ? (streaming ? adamw_many_kernel<32, true> : adamw_many_kernel<32, false>)
-                         : (streaming ? adamw_many_kernel<8, true> : adamw_many_kernel<8, false>);
-    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, s, a);
+    if (list == 0) return streaming ? adamw_many_kernel<BITS, 0, true> : adamw_many_kernel<BITS, 0, false>;
+    if (list == 1) return streaming ? adamw_many_kernel<BITS, 1, true> : adamw_many_kernel<BITS, 1, false>;
+    return streaming ? adamw_many_kernel<BITS, 2, true> : adamw_many_kernel<BITS, 2, false>;
+}
+
+hipError_t launch_adamw_many(const AdamWArgs& a, int bits, int list, bool streaming, uint32_t blocks, hipStream_t s)
+{
+    auto* k = bits == 32 ? adamw_kernel_of<32>(list, streaming) : adamw_kernel_of<8>(list, streaming);
+    // Past the caches fewer workgroups at a time are faster: each has four streams that it reads and writes, and the fewer there are
+    // the longer memory stays with one.  LDS that nobody uses keeps it at three to a CU.  Measured with 6 (8 for 32 bits) | 5 | 3 |
+    // 2 a CU, us: 8 bits 100M fp32 parameters with clipping 373 | 360 | 356 | 379; 32 bits 268M fp32 1320 | 1308 | 1308 | 1297, 40M bf16
+    // 164.5 | 162.3 | 161.6 | 158.6.  8 bits with bf16 parameters, where arithmetic takes the time, want all they can get: 268M
+    // parameters 483 | 494 | 513 | 601.
+    const unsigned idle_lds = streaming && !(bits == 8 && list == 1) ? 53000 : 0;
+    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), idle_lds, s, a);
     return hipGetLastError();
 }
 
