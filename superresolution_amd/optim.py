@@ -542,13 +542,16 @@ class AdamW(torch.optim.Optimizer):
         for group, mo, saved in zip(self.param_groups, self.moments, groups):
             m = torch.zeros(mo.total, dtype=torch.float32, device=mo.device)
             v = torch.zeros_like(m)
-            steps = []
+            steps, into, values = [], [], []
             for i, (p, key) in enumerate(zip(group["params"], saved["params"])):
                 st = state.get(key)
                 steps.append(0 if st is None else int(float(st["step"])))
                 if st is not None:
                     for x, name in ((m, "exp_avg"), (v, "exp_avg_sq")):
-                        torch.as_strided(x, p.shape, p.stride(), mo.offsets[i]).copy_(st[name].reshape(p.shape))
+                        into.append(torch.as_strided(x, p.shape, p.stride(), mo.offsets[i]))
+                        values.append(st[name].detach().reshape(p.shape))
+            if into:
+                torch._foreach_copy_(into, values)
             if steps:
                 mo.set_steps(steps)
             mo.write(m, v)
