@@ -7,7 +7,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <utility>
+#include <vector>
 
 namespace {
 
@@ -117,6 +120,29 @@ PyObject* tensors_impl(PyObject* args)
     Py_RETURN_TRUE;
 }
 
+// apart(n, ptr, numel, code) -> True if no two of the tensors share memory
+PyObject* apart_impl(PyObject* args)
+{
+    PyObject* o[3];
+    Py_ssize_t n;
+    if (!PyArg_ParseTuple(args, "nOOO", &n, &o[0], &o[1], &o[2])) return nullptr;
+    if (n < 0) {
+        PyErr_SetString(PyExc_ValueError, "negative count");
+        return nullptr;
+    }
+    Buffer ptr(o[0], n, 8), numel(o[1], n, 8), code(o[2], n, 4);
+    if (!ptr.ok || !numel.ok || !code.ok) return nullptr;
+    std::vector<std::pair<uint64_t, uint64_t>> spans;
+    spans.reserve((size_t)n);
+    for (Py_ssize_t i = 0; i < n; ++i)
+        if (const uint64_t bytes = numel.as<uint64_t>()[i] * (code.as<int32_t>()[i] == 0 ? 4 : 2))
+            spans.emplace_back(ptr.as<uint64_t>()[i], ptr.as<uint64_t>()[i] + bytes);
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        if (spans[i].first < spans[i - 1].second) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
+}
+
 // bump(list, g): version counters of the tensors that were written (those with g[i] != 0; g = None: all)
 PyObject* bump_impl(PyObject* args)
 {
@@ -146,10 +172,12 @@ PyObject* bump_impl(PyObject* args)
 
 PyObject* params(PyObject*, PyObject* args) { return guarded(params_impl, args); }
 PyObject* tensors(PyObject*, PyObject* args) { return guarded(tensors_impl, args); }
+PyObject* apart(PyObject*, PyObject* args) { return guarded(apart_impl, args); }
 PyObject* bump(PyObject*, PyObject* args) { return guarded(bump_impl, args); }
 
 PyMethodDef methods[] = {{"params", params, METH_VARARGS, "addresses and types of parameters and their gradients"},
                          {"tensors", tensors, METH_VARARGS, "addresses, sizes and types of tensors"},
+                         {"apart", apart, METH_VARARGS, "whether no two tensors share memory"},
                          {"bump", bump, METH_VARARGS, "version counters of written tensors"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -93,13 +93,10 @@ def _one_device(tensors, what: str) -> torch.device:
     return next(iter(devs))
 
 
-def _no_overlap(spans, what: str) -> None:
-    """``spans``: (address, bytes) of tensors that are written."""
-    end = 0
-    for a, n in sorted(s for s in spans if s[1]):
-        if a < end:
-            raise RuntimeError(f"{what}: two of the tensors share memory (the same one twice?)")
-        end = a + n
+def _no_overlap(ptr: array, numel: array, code: array, what: str) -> None:
+    """Refuses a list of tensors that are written where two of them share memory."""
+    if not _tensorlist.apart(len(ptr), ptr, numel, code):
+        raise RuntimeError(f"{what}: two of the tensors share memory (the same one twice?)")
 
 
 # ---- moments -----------------------------------------------------------------------------------------------------------
@@ -305,7 +302,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     for g, t in zip(grads, listed):
         if g is not t:
             raise RuntimeError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or overlaps")
-    _no_overlap([(a, n * (4 if c == _lib.SRGEN_F32 else 2)) for a, n, c in zip(ptr, numel, code)], "clip_grad_norm_")
+    _no_overlap(ptr, numel, code, "clip_grad_norm_")
     out = _norm_coef(dev, ptr, numel, code, float(max_norm))[-2:]
     if error_if_nonfinite and not bool(torch.isfinite(out[0])):
         raise RuntimeError("The total norm of order 2.0 for gradients from `parameters` is non-finite, so it cannot be clipped. To "
@@ -391,7 +388,7 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()} has gaps or overlaps")
             if len({id(p) for p in g["params"]}) != len(g["params"]):
                 raise ValueError("AdamW: a parameter appears twice in a group")
-            _no_overlap([(p.data_ptr(), p.numel() * p.element_size()) for h in self.param_groups for p in h["params"]], "AdamW")
+            self._check_memory()
         except Exception:
             self.param_groups.pop()
             raise
@@ -501,9 +498,15 @@ class AdamW(torch.optim.Optimizer):
 
     def _check_memory(self) -> None:
         """No two parameters share memory: looked at when their addresses are not those that were looked at last."""
-        _no_overlap([(p.data_ptr(), p.numel() * p.element_size()) for h in self.param_groups for p in h["params"]], "AdamW")
-        for h, ls in zip(self.param_groups, self._lists):
-            ls.checked = array("Q", map(_data_ptr, h["params"])), _codes(h["params"], "AdamW")
+        seen = [(array("Q", map(_data_ptr, h["params"])), array("Q", map(_numel, h["params"])), _codes(h["params"], "AdamW"))
+                for h in self.param_groups]
+        every = [array(t) for t in "QQi"]
+        for ptr, numel, code in seen:
+            for a, b in zip(every, (ptr, numel, code)):
+                a.extend(b)
+        _no_overlap(*every, "AdamW")
+        for ls, (ptr, _, code) in zip(self._lists, seen):
+            ls.checked = ptr, code
 
     # -- checkpoints --------------------------------------------------------------------------------------------------
     def state_dict(self) -> dict:

@@ -143,9 +143,13 @@ def test_dense_and_overlap_checks():
     assert _dense(t) and _dense(t.to(memory_format=torch.channels_last)) and _dense(t.permute(3, 1, 0, 2)) and _dense(torch.zeros(3, 0))
     assert not _dense(t[:, ::2]) and not _dense(torch.zeros(1).expand(4)) and not _dense(t[:, :5])
     assert _dense(t[1:3]) and _dense(torch.zeros(()))
-    _no_overlap([(0, 8), (16, 8), (8, 8), (4, 0)], "x")
+    _no_overlap(array("Q", [0, 16, 8, 4]), array("Q", [2, 2, 4, 0]), array("i", [0, 0, 1, 0]), "x")
     with pytest.raises(RuntimeError, match="share memory"):
-        _no_overlap([(0, 8), (4, 8)], "x")
+        _no_overlap(array("Q", [0, 4]), array("Q", [2, 2]), array("i", [0, 0]), "x")
+    with pytest.raises(RuntimeError, match="share memory"):
+        _no_overlap(array("Q", [64, 64]), array("Q", [1, 1]), array("i", [1, 2]), "x")
+    with pytest.raises(ValueError):
+        _no_overlap(array("Q", [64, 128]), array("Q", [1]), array("i", [1, 2]), "x")
 
 
 def test_oracle_against_torch_adamw():
