@@ -51,19 +51,31 @@ int check_list(int count, const void* const* t, const uint64_t* numel, const int
     return SRGEN_OK;
 }
 
-inline OptTensor list_entry(const void* t, uint64_t numel, int32_t dtype, uint64_t block0)
-{
-    return OptTensor{(uint64_t)(uintptr_t)t | (uint64_t)dtype << 48 | (numel >> 32) << 52, (uint32_t)numel, (uint32_t)block0};
-}
-
-// elements of one workgroup of the norm: more for long lists, so that the partial sums stay few enough for one workgroup to add
-uint32_t norm_per_block(int count, const uint64_t* numel)
+// elements of one workgroup of the norm: more for long lists, so that the partial sums stay few
+uint32_t norm_part(int count, const uint64_t* numel)
 {
     uint64_t total = 0;
     for (int i = 0; i < count; ++i) total += numel[i];
-    uint64_t per = kOptChunk;
-    while (per < (1u << 20) && total / per > 8192) per *= 2;
-    return (uint32_t)per;
+    uint32_t per = kOptChunk;
+    while (per < kOptMaxPart && total / per > 8192) per *= 2;
+    return per;
+}
+
+// takes tensors from *i on into one launch, until its descriptors or its workgroups are full; the number of its workgroups
+uint32_t fill_list(int count, const void* const* t, const uint64_t* numel, const int32_t* dtype, int* i, OptTensors* ts)
+{
+    uint64_t blocks = 0;
+    ts->count = 0;
+    for (; *i < count && ts->count < kOptMaxListed; ++*i) {
+        const uint64_t n = t[*i] ? numel[*i] : 0, c = chunks_of(n, ts->part);
+        if (blocks + c > kMaxBlocks) break;
+        if (!c) continue;
+        ts->t[ts->count] = (uint64_t)(uintptr_t)t[*i] | (uint64_t)dtype[*i] << 48 | (n - (c - 1) * ts->part - 1) << 50;
+        ts->block0[ts->count++] = (uint32_t)blocks;
+        blocks += c;
+    }
+    ts->block0[ts->count] = (uint32_t)blocks;
+    return (uint32_t)blocks;
 }
 
 // the partial sums of the list's squares (tensors with g[i] == NULL are left out); the list has been checked
@@ -71,7 +83,7 @@ int norm_partials(int count, const void* const* g, const uint64_t* numel, const 
                   size_t scratch_bytes, void* stream, uint32_t* partials)
 {
     if (!norm_coef2 || !aligned(norm_coef2, 4)) return fail(SRGEN_E_INVALID, "norm_coef2 is NULL or misaligned");
-    const uint32_t per = norm_per_block(count, numel);
+    const uint32_t per = norm_part(count, numel);
     uint64_t total = 0, bytes = 0;
     for (int i = 0; i < count; ++i) {
         if (!g[i]) continue;
@@ -83,20 +95,12 @@ int norm_partials(int count, const void* const* g, const uint64_t* numel, const 
     if (scratch_bytes < total * sizeof(double))
         return fail(SRGEN_E_WORKSPACE, "scratch of %zu bytes, %zu needed", scratch_bytes, (size_t)total * sizeof(double));
     OptTensors ts;
-    uint64_t done = 0;
+    ts.part = per;
+    ts.partial0 = 0;
     for (int i = 0; i < count;) {
-        uint64_t blocks = 0;
-        ts.count = 0;
-        for (; i < count && ts.count < kOptMaxTensors; ++i) {
-            const uint64_t c = g[i] ? chunks_of(numel[i], per) : 0;
-            if (blocks + c > kMaxBlocks) break;
-            if (!c) continue;
-            ts.t[ts.count++] = list_entry(g[i], numel[i], dtype[i], blocks);
-            blocks += c;
-        }
-        ts.partial0 = (uint32_t)done;
-        done += blocks;
-        if (blocks) HIP_TRY(launch_norm_partial(ts, bytes > kStreamingNormBytes, (uint32_t)blocks, per, (double*)scratch, (hipStream_t)stream));
+        const uint32_t blocks = fill_list(count, g, numel, dtype, &i, &ts);
+        if (blocks) HIP_TRY(launch_norm_partial(ts, bytes > kStreamingNormBytes, blocks, (double*)scratch, (hipStream_t)stream));
+        ts.partial0 += blocks;
     }
     *partials = (uint32_t)total;
     return SRGEN_OK;
@@ -193,8 +197,11 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
         for (; i < count && k < kOptMaxTensors; ++i, ++k) {
             const uint64_t c = chunks_of(numel[i], kOptChunk);
             if (blocks + c > kMaxBlocks) break;
-            a.p[k] = (uint64_t)(uintptr_t)p[i] | (uint64_t)p_dtype[i] << 48;
-            a.g[k] = g[i] ? (uint64_t)(uintptr_t)g[i] | (uint64_t)g_dtype[i] << 48 : 0;
+            const uint64_t pa = (uint64_t)(uintptr_t)p[i] | (p_dtype[i] == SRGEN_BF16);
+            const uint64_t ga = g[i] ? (uint64_t)(uintptr_t)g[i] | (g_dtype[i] == SRGEN_BF16) : 0;
+            a.p[k] = (uint32_t)pa;
+            a.g[k] = (uint32_t)ga;
+            a.hi[k] = (uint32_t)(pa >> 32) | (uint32_t)(ga >> 32) << 16;
             any |= g[i] && c;
             blocks += c;
         }
@@ -208,7 +215,7 @@ int srgen_adamw_many(int count, void* const* p, const void* const* g, const uint
 int srgen_total_norm_scratch_bytes(int count, const uint64_t* numel, size_t* bytes)
 {
     if (count < 0 || (count && !numel) || !bytes) return fail(SRGEN_E_INVALID, "NULL argument or count %d", count);
-    const uint32_t per = norm_per_block(count, numel);
+    const uint32_t per = norm_part(count, numel);
     uint64_t n = 0;
     for (int i = 0; i < count; ++i) n += chunks_of(numel[i], per);
     *bytes = (size_t)((n * sizeof(double) + 255) & ~(uint64_t)255);
@@ -229,21 +236,14 @@ int srgen_scale_many(int count, void* const* g, const uint64_t* numel, const int
 {
     if (int rc = check_list(count, g, numel, dtype, "tensor", true)) return rc;
     if (!coef) return fail(SRGEN_E_INVALID, "coef is NULL");
-    OptTensors ts;
-    ts.partial0 = 0;
     for (int i = 0; i < count; ++i)
         if (numel[i] && !g[i]) return fail(SRGEN_E_INVALID, "tensor %d is NULL", i);
+    OptTensors ts;
+    ts.part = kOptChunk;
+    ts.partial0 = 0;
     for (int i = 0; i < count;) {
-        uint64_t blocks = 0;
-        ts.count = 0;
-        for (; i < count && ts.count < kOptMaxTensors; ++i) {
-            const uint64_t c = chunks_of(numel[i], kOptChunk);
-            if (blocks + c > kMaxBlocks) break;
-            if (!c) continue;
-            ts.t[ts.count++] = list_entry(g[i], numel[i], dtype[i], blocks);
-            blocks += c;
-        }
-        if (blocks) HIP_TRY(launch_scale_many(ts, (uint32_t)blocks, coef, (hipStream_t)stream));
+        const uint32_t blocks = fill_list(count, g, numel, dtype, &i, &ts);
+        if (blocks) HIP_TRY(launch_scale_many(ts, blocks, coef, (hipStream_t)stream));
     }
     return SRGEN_OK;
 }

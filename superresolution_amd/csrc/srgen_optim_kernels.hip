@@ -539,12 +539,13 @@ __global__ __launch_bounds__(256) void adamw_many_kernel(const AdamWArgs a)
 {
     __shared__ StepScalars shared;
     const OptChunk ck = a.mo.chunks[a.chunk0 + blockIdx.x];
-    const uint64_t pw = a.p[ck.tensor - a.tensor0], gw = a.g[ck.tensor - a.tensor0];
+    const uint32_t at = ck.tensor - a.tensor0, hi = a.hi[at];
+    const uint64_t pw = a.p[at] | (uint64_t)(hi & 0xFFFFu) << 32, gw = a.g[at] | (uint64_t)(hi >> 16) << 32;
     if (gw == 0) return;
     if (a.sc.found_inf && *a.sc.found_inf != 0.f) return;
-    const int pdt = LIST == 2 ? (int)(pw >> 48) : LIST, gdt = LIST == 2 ? (int)(gw >> 48) : LIST;
+    const int pdt = LIST == 2 ? (int)(pw & 1) : LIST, gdt = LIST == 2 ? (int)(gw & 1) : LIST;
     const uint64_t base = (uint64_t)ck.index * kOptChunk, off = (uint64_t)ck.offset32 * kOptBlock;
-    const Chunk c{(void*)((pw & kAddrMask) + base * (pdt ? 2 : 4)), (const void*)((gw & kAddrMask) + base * (gdt ? 2 : 4)),
+    const Chunk c{(void*)((pw & ~1ull) + base * (pdt ? 2 : 4)), (const void*)((gw & ~1ull) + base * (gdt ? 2 : 4)),
                   (uint8_t*)a.mo.m + off * (BITS / 8), (uint8_t*)a.mo.v + off * (BITS / 8), a.mo.m_scale + ck.offset32, a.mo.v_scale + ck.offset32,
                   ck.count, round_up_block(ck.count), (uint32_t)off, (uint32_t)off + (uint32_t)(off >> 32) * kGold, ck.index == 0};
     if constexpr (LIST == 0) adamw_chunk_any<BITS, 0, 0, 4, NT>(a, c, &shared);
@@ -558,27 +559,28 @@ __global__ __launch_bounds__(256) void adamw_many_kernel(const AdamWArgs a)
     }
 }
 
-// which tensor of a launch a workgroup works on (the last one with block0 <= blk), its element type and size
+// which part of which tensor a workgroup works on
 struct Found {
-    const char* base;
-    uint64_t n;
+    const char* base;       // of the part
+    uint32_t n;             // its elements
     int dt;
-    uint32_t block;         // in the tensor
 };
-// (every wave counts the tensors that start at or before the workgroup: four loads at once instead of eight one after another)
-__device__ inline Found find_tensor(const OptTensors& ts, uint32_t blk)
+// (every wave counts the tensors that start at or before the workgroup: its loads go out at once, a search's would follow each other)
+__device__ inline Found find_part(const OptTensors& ts, uint32_t blk)
 {
-    static_assert(kOptMaxTensors <= 256, "four entries a lane");
     const int lane = threadIdx.x & 63;
     int at = -1;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < (kOptMaxListed + 63) / 64; ++u) {
         const int k = lane + 64 * u;
-        const uint32_t first = ts.t[k < kOptMaxTensors ? k : 0].block0;
+        const uint32_t first = ts.block0[k < kOptMaxListed ? k : 0];
         at += __popcll(__ballot(k < ts.count && first <= blk));
     }
-    const OptTensor& t = ts.t[__builtin_amdgcn_readfirstlane(at)];
-    return Found{(const char*)(t.ptr & kAddrMask), t.numel_lo | (t.ptr >> 52) << 32, (int)(t.ptr >> 48) & 15, blk - t.block0};
+    at = __builtin_amdgcn_readfirstlane(at);
+    const uint64_t t = ts.t[at];
+    const int dt = (int)(t >> 48) & 3;
+    return Found{(const char*)(t & kAddrMask) + (uint64_t)(blk - ts.block0[at]) * ts.part * (dt == 0 ? 4 : 2),
+                 blk + 1 == ts.block0[at + 1] ? (uint32_t)(t >> 50) + 1 : ts.part, dt};
 }
 
 // ---- total norm --------------------------------------------------------------------------------------------------------
@@ -593,7 +595,7 @@ struct Vec16 {
         h8 h;
     };
     template <bool NT>
-    __device__ inline void load(const void* p, uint64_t i)
+    __device__ inline void load(const void* p, uint32_t i)
     {
         if constexpr (DT == 0) f = load_as<NT>((const GLOBAL f4*)((const GLOBAL float*)p + i));
         else h = load_as<NT>((const GLOBAL h8*)((const GLOBAL unsigned short*)p + i));
@@ -610,26 +612,26 @@ struct Vec16 {
 };
 
 template <int DT, bool NT>
-__device__ inline double sum_squares(const void* p, uint64_t base, uint64_t end)
+__device__ inline double sum_squares(const void* p, uint32_t n)
 {
     constexpr int N = Vec16<DT>::N, U = 4;                 // four loads of 16 bytes requested before the first is used
     constexpr uint32_t STEP = 256 * N;
     double acc = 0.0;
-    uint64_t i = base + threadIdx.x * N;
-    for (; i + (U - 1) * STEP + N <= end; i += U * STEP) {
+    uint32_t i = threadIdx.x * N;
+    for (; i + (U - 1) * STEP + N <= n; i += U * STEP) {
         Vec16<DT> x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) x[u].template load<NT>(p, i + u * STEP);
 #pragma unroll
         for (int u = 0; u < U; ++u) acc = x[u].add(acc);
     }
-    for (; i < end; i += STEP) {
-        if (i + N <= end) {
+    for (; i < n; i += STEP) {
+        if (i + N <= n) {
             Vec16<DT> x;
             x.template load<NT>(p, i);
             acc = x.add(acc);
         } else {
-            for (uint64_t k = i; k < end; ++k) {
+            for (uint32_t k = i; k < n; ++k) {
                 const double x = DT == 0 ? (double)((const GLOBAL float*)p)[k]
                                : DT == 1 ? (double)bf16_to_f32(((const GLOBAL unsigned short*)p)[k])
                                          : (double)(float)__builtin_bit_cast(_Float16, ((const GLOBAL unsigned short*)p)[k]);
@@ -642,18 +644,14 @@ __device__ inline double sum_squares(const void* p, uint64_t base, uint64_t end)
 
 // Sums of squares in 64 bits, in a fixed order: one partial sum for each workgroup's elements.  One pass over the gradients, bound by
 // memory: 73M fp32 in 44.6 us = 6.5 TB/s, 66M bf16 in 26 to 30 us = 4.4 to 5.1 TB/s (16 KB to 64 KB a workgroup: at most 8,192 partial sums is the
-// best of 1,024 to 32,768: 86, 67, 61, 57, 60, 71 us for 120M bf16 values in three launches).  Eight loads in flight instead of four
-// halve the occupancy (57 -> 60 us).
+// best of 1,024 to 32,768: 86, 67, 61, 57, 60, 71 us for 120M bf16 values in 500 tensors when they took three launches; 50 us in
+// two).  Eight loads in flight instead of four halve the occupancy (57 -> 60 us).
 template <bool NT>
-__global__ __launch_bounds__(256) void norm_partial_kernel(const OptTensors ts, uint32_t per_block, double* __restrict__ partial)
+__global__ __launch_bounds__(256) void norm_partial_kernel(const OptTensors ts, double* __restrict__ partial)
 {
     __shared__ double red[4];
-    const Found f = find_tensor(ts, blockIdx.x);
-    const uint64_t base = (uint64_t)f.block * per_block;
-    const uint64_t end = base + per_block < f.n ? base + per_block : f.n;
-    double acc = f.dt == 0 ? sum_squares<0, NT>(f.base, base, end)
-               : f.dt == 1 ? sum_squares<1, NT>(f.base, base, end)
-                           : sum_squares<2, NT>(f.base, base, end);
+    const Found f = find_part(ts, blockIdx.x);
+    double acc = f.dt == 0 ? sum_squares<0, NT>(f.base, f.n) : f.dt == 1 ? sum_squares<1, NT>(f.base, f.n) : sum_squares<2, NT>(f.base, f.n);
     acc = wave_sum(acc);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
     __syncthreads();
@@ -695,10 +693,9 @@ __global__ __launch_bounds__(256) void scale_many_kernel(const OptTensors ts, co
 {
     const float c = *coef;
     if (c == 1.f) return;
-    const Found f = find_tensor(ts, blockIdx.x);
-    const uint64_t base = (uint64_t)f.block * kOptChunk, left = f.n - base;
-    const uint32_t n = left < kOptChunk ? (uint32_t)left : kOptChunk;
-    void* const q0 = (void*)(f.base + base * (f.dt == 0 ? 4 : 2));
+    const Found f = find_part(ts, blockIdx.x);
+    const uint32_t n = f.n;
+    void* const q0 = (void*)f.base;
     for (uint32_t i = threadIdx.x * 4; i < n; i += 1024) {
         float g[4];
         if (f.dt == 0) load_elements<0, 4, false, false>(q0, i, n).values(g);
@@ -783,10 +780,10 @@ hipError_t launch_adamw_many(const AdamWArgs& a, int bits, int list, bool stream
     return hipGetLastError();
 }
 
-hipError_t launch_norm_partial(const OptTensors& ts, bool streaming, uint32_t blocks, uint32_t per_block, double* partial, hipStream_t s)
+hipError_t launch_norm_partial(const OptTensors& ts, bool streaming, uint32_t blocks, double* partial, hipStream_t s)
 {
     auto* k = streaming ? norm_partial_kernel<true> : norm_partial_kernel<false>;
-    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, s, ts, per_block, partial);
+    hipLaunchKernelGGL(k, dim3(blocks), dim3(256), 0, s, ts, partial);
     return hipGetLastError();
 }
 
