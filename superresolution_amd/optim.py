@@ -405,10 +405,16 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None):
         # torch wraps the step() of every optimizer in a profiler range and its hooks, which takes longer than a small step does:
         # here only where a profiler runs or somebody has registered a hook
-        if (torch._C._autograd._profiler_enabled() or self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks
-                or any(_GLOBAL_HOOKS)):
-            return self._step_with_hooks(closure)
-        return self._step(closure)
+        try:
+            if (torch._C._autograd._profiler_enabled() or self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks
+                    or any(_GLOBAL_HOOKS)):
+                return self._step_with_hooks(closure)
+            return self._step(closure)
+        except BaseException:
+            # GradScaler takes these back only after a step that returns: a later step would divide by this one's scale
+            self.__dict__.pop("grad_scale", None)
+            self.__dict__.pop("found_inf", None)
+            raise
 
     step.hooked = True                                     # (how torch's wrapper marks the ones it has wrapped)
 

@@ -252,6 +252,36 @@ def test_grad_scaler_drives_it():
     assert opt.moments[0].steps() == [2, 2]
 
 
+def test_grad_scaler_and_clipping():
+    """Clipping inside the step wants unscaled gradients: refused otherwise, and the skipped step still tells its norm."""
+    from superresolution_amd import optim
+    torch.manual_seed(0)
+    model = torch.nn.Linear(16, 4).cuda()
+    twin = torch.nn.Linear(16, 4).cuda()
+    twin.load_state_dict(model.state_dict())
+    opt, ref = (optim.AdamW(m.parameters(), lr=1e-2, max_grad_norm=0.1) for m in (model, twin))
+    scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 12)
+    x = torch.randn(8, 16, device="cuda")
+    scaler.scale(model(x).square().mean()).backward()
+    with pytest.raises(RuntimeError, match="unscale_"):
+        scaler.step(opt)
+    opt.zero_grad()
+    scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 12)
+    for k in range(3):
+        opt.zero_grad()
+        ref.zero_grad()
+        scaler.scale(model(x).square().mean() * (float("nan") if k == 1 else 1.0)).backward()
+        scaler.unscale_(opt)
+        scaler.step(opt)
+        scaler.update()
+        if k != 1:
+            twin(x).square().mean().backward()
+            ref.step()
+            assert torch.equal(model.weight, twin.weight) and torch.equal(opt.last_grad_norm, ref.last_grad_norm)
+        else:
+            assert torch.isnan(opt.last_grad_norm)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("lr", [0.0, 1e-44, 1e-39, 1e-30])
 def test_vanishing_learning_rates_and_zero_gradients(bits, lr):
