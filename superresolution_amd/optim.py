@@ -455,23 +455,26 @@ class AdamW(torch.optim.Optimizer):
                     g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
                 self._norm_coef = _norm_coef(dev, g, numel, code, self.max_grad_norm)
                 mul = self._norm_coef.data_ptr() + 4 * (self._norm_coef.numel() - 1)
+        calls = []                                         # (all of them before the first: no group steps if another is refused)
+        for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
+            if not n:
+                continue
+            lr, (b1, b2) = group["lr"], group["betas"]
+            lr_dev = None
+            if isinstance(lr, torch.Tensor):
+                if lr.is_cuda:
+                    if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
+                        raise RuntimeError(f"AdamW: a learning rate on the device is an fp32 scalar on {dev}")
+                    lr_dev, lr = lr.data_ptr(), 0.0
+                else:
+                    lr = float(lr)
+            calls.append((group, mo, ls, _lib.srgen_adamw_args(
+                lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, mul, None if div is None else div.data_ptr(),
+                None if found is None else found.data_ptr(), out, scratch, mo.norm_bytes, self.max_grad_norm or 0.0, self.seed,
+                1 if group["maximize"] else 0)))
         with _on(dev):
             stream = _stream(dev)
-            for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
-                if not n:
-                    continue
-                lr, (b1, b2) = group["lr"], group["betas"]
-                lr_dev = None
-                if isinstance(lr, torch.Tensor):
-                    if lr.is_cuda:
-                        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev:
-                            raise RuntimeError(f"AdamW: a learning rate on the device is an fp32 scalar on {dev}")
-                        lr_dev, lr = lr.data_ptr(), 0.0
-                    else:
-                        lr = float(lr)
-                args = _lib.srgen_adamw_args(lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, mul, None if div is None else div.data_ptr(),
-                                             None if found is None else found.data_ptr(), out, scratch, mo.norm_bytes,
-                                             self.max_grad_norm or 0.0, self.seed, 1 if group["maximize"] else 0)
+            for group, mo, ls, args in calls:
                 mo._update(ls.pg, ls.codes, args, stream)
                 # the kernel wrote behind torch's back: the version counters are what the Generator / Discriminator mirrors
                 # watch to upload their weights again

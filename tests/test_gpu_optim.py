@@ -282,6 +282,20 @@ def test_grad_scaler_and_clipping():
             assert torch.isnan(opt.last_grad_norm)
 
 
+def test_a_refused_group_keeps_the_others_from_stepping():
+    from superresolution_amd import optim
+    a, b = (torch.nn.Parameter(torch.ones(40, device="cuda")) for _ in range(2))
+    opt = optim.AdamW([{"params": [a]}, {"params": [b]}], lr=1e-2)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt.param_groups[1]["lr"] = torch.tensor(1e-2, dtype=torch.float64, device="cuda")
+    with pytest.raises(RuntimeError, match="fp32 scalar"):
+        opt.step()
+    assert torch.equal(a, torch.ones_like(a)) and opt.moments[0].steps() == [0]
+    opt.param_groups[1]["lr"] = torch.tensor(1e-2, device="cuda")
+    opt.step()
+    assert torch.equal(a, b) and not torch.equal(a, torch.ones_like(a))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("lr", [0.0, 1e-44, 1e-39, 1e-30])
 def test_vanishing_learning_rates_and_zero_gradients(bits, lr):
