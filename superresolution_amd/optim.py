@@ -172,6 +172,10 @@ class Moments:
 
     def update(self, p: array, g: array, p_dtype: array, g_dtype: array, args: "_lib.srgen_adamw_args", stream: int) -> None:
         """One AdamW step of the list (addresses and type codes in the list's order; address 0: no gradient)."""
+        if not len(p) == len(g) == len(p_dtype) == len(g_dtype) == len(self.numels):
+            raise ValueError(f"Moments.update: an address and a type code for each of the {len(self.numels)} tensors")
+        if (p.typecode, g.typecode, p_dtype.typecode, g_dtype.typecode) != ("Q", "Q", "i", "i"):
+            raise TypeError("Moments.update: addresses as array('Q'), type codes as array('i')")
         self._update((_addr(p), _addr(g)), (_addr(p_dtype), _addr(g_dtype)), args, stream)
 
     def _update(self, pg, codes, args, stream: int) -> None:

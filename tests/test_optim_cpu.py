@@ -184,3 +184,20 @@ def test_oracle_e4m3_is_torchs_format_and_unbiased():
     # the mean of 400 roundings of variance <= step^2 / 4: five standard deviations, over 2,048 elements (p < 2e-3), plus the
     # 2^-16 of a step that 16 random bits do not resolve
     assert (np.abs(mean - x) <= step * (5 * 0.5 / np.sqrt(rounds) + 2.0 ** -16)).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_update_refuses_other_lists(bits):
+    """Arrays that are not one entry for each tensor, or of another type, would be read past their end."""
+    from array import array
+    from superresolution_amd import _lib, optim
+    mo = optim.Moments([5, 40], bits, torch.device("cpu"))
+    q, i, args = array("Q", [0, 0]), array("i", [0, 0]), _lib.srgen_adamw_args()
+    for k in range(4):
+        lists = [q, q, i, i]
+        lists[k] = lists[k][:1]
+        with pytest.raises(ValueError, match="2 tensors"):
+            mo.update(*lists, args, 0)
+        lists[k] = array("I", [0, 0]) if k < 2 else array("h", [0, 0])
+        with pytest.raises(TypeError, match="type codes"):
+            mo.update(*lists, args, 0)
