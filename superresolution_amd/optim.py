@@ -29,7 +29,6 @@ from torch.optim import optimizer as _torch_optimizer
 from . import _lib
 
 
-
 class _NotBuilt:
     """Stands for an extension that is missing (the package can be imported to build it): raises where it is used."""
 
@@ -272,8 +271,8 @@ def _norm_coef(dev: torch.device, ptr: array, numel: array, code: array, max_nor
 
 def total_norm(tensors) -> torch.Tensor:
     """The L2 norm of all ``tensors`` (fp32, bf16, fp16) taken together, as a 0-dim fp32 device tensor
-    (``torch.nn.utils.get_total_norm``; not differentiable).  Sums are held in 64 bits and added in a fixed order: the result does not overflow
-    before the norm itself does, and repeats bit for bit."""
+    (``torch.nn.utils.get_total_norm``; not differentiable).  Sums are held in 64 bits and added in a fixed order: the result does
+    not overflow before the norm itself does, and repeats bit for bit."""
     ts = _tensor_list(tensors)
     if not ts:
         return torch.tensor(0.0)
@@ -294,9 +293,11 @@ def grad_norm(model) -> torch.Tensor:
 
 
 @torch.no_grad()
-def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
-    """``torch.nn.utils.clip_grad_norm_`` (``train.py:175``): scales the gradients in place so that their total L2 norm is at
-    most ``max_norm``; returns the norm before.  ``AdamW(max_grad_norm=...)`` clips without the extra pass."""
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                    foreach: Optional[bool] = None) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` (``train.py:175``): scales the gradients (of one device) in place so that their total L2
+    norm is at most ``max_norm``; returns the norm before.  ``foreach`` is taken and has no meaning here.
+    ``AdamW(max_grad_norm=...)`` clips without the extra pass."""
     if float(norm_type) != 2.0:
         raise NotImplementedError(f"clip_grad_norm_: the L2 norm only, got norm_type={norm_type}")
     grads = _grads(parameters)
@@ -358,7 +359,8 @@ class AdamW(torch.optim.Optimizer):
     then follows it.  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
     optimizer have to stay.  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
     gradient does not happen.  ``state_dict`` has the layout of ``torch.optim.AdamW`` with fp32 moments, whatever
-    ``state_bits``: checkpoints move between the two, and between 8 and 32 bits.
+    ``state_bits``: checkpoints move between the two, and between 8 and 32 bits (``state`` stays empty: ``moments`` has one
+    ``Moments`` for each group).
 
     The random bits do not depend on the process: data-parallel ranks that take the same gradients stay the same bit for bit.
     A second moment beyond fp32's range (gradients of some 1e20) is infinite with 32 bits, which stops the element, and NaN with

@@ -296,6 +296,27 @@ def test_a_refused_group_keeps_the_others_from_stepping():
     assert torch.equal(a, b) and not torch.equal(a, torch.ones_like(a))
 
 
+def test_hooks_and_profiler_see_the_step():
+    from torch.optim.optimizer import register_optimizer_step_post_hook
+    from superresolution_amd import optim
+    p = torch.nn.Parameter(torch.ones(40, device="cuda"))
+    opt = optim.AdamW([p], lr=1e-2)
+    p.grad = torch.ones_like(p)
+    seen = []
+    pre = opt.register_step_pre_hook(lambda o, a, k: seen.append("pre"))
+    post = opt.register_step_post_hook(lambda o, a, k: seen.append("post"))
+    opt.step()
+    assert seen == ["pre", "post"]
+    pre.remove()
+    post.remove()
+    everywhere = register_optimizer_step_post_hook(lambda o, a, k: seen.append("all"))
+    opt.step()
+    everywhere.remove()
+    assert seen == ["pre", "post", "all"]
+    loss = opt.step(lambda: (p * 2.0).sum())
+    assert float(loss) > 0 and len(seen) == 3 and opt.moments[0].steps() == [3]
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("lr", [0.0, 1e-44, 1e-39, 1e-30])
 def test_vanishing_learning_rates_and_zero_gradients(bits, lr):
