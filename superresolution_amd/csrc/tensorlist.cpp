@@ -49,12 +49,13 @@ int type_code(const at::Tensor& t)            // SRGEN_F32, SRGEN_BF16, SRGEN_F1
     }
 }
 
-// strided, contiguous, on the device, of a known type: what a kernel may walk from its first address
+// strided, contiguous, on the device, of a known type, with memory of its own (a wrapping subclass has none) that holds its
+// values (a lazily negated view's does not): what a kernel may walk from its first address
 bool plain(const at::Tensor& t, int device, int max_code, int* code)
 {
     if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device) return false;
     *code = type_code(t);
-    return *code >= 0 && *code <= max_code && t.is_contiguous();
+    return *code >= 0 && *code <= max_code && t.is_contiguous() && !t.is_neg() && (t.numel() == 0 || t.data_ptr() != nullptr);
 }
 
 PyObject* guarded(PyObject* (*f)(PyObject*), PyObject* args)
@@ -77,6 +78,7 @@ PyObject* params_impl(PyObject* args)
     const Py_ssize_t n = PyList_GET_SIZE(list);
     Buffer numel(o[0], n, 8), p(o[1], n, 8), pc(o[2], n, 4), g(o[3], n, 8), gc(o[4], n, 4);
     if (!numel.ok || !p.ok || !pc.ok || !g.ok || !gc.ok) return nullptr;
+    if (numel.b.len != n * 8) return PyLong_FromLong(-1);  // (what the arrays hold of parameters that are gone is stale)
     long grads = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
         PyObject* x = PyList_GET_ITEM(list, i);

@@ -85,6 +85,14 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _own_memory(tensors, what: str) -> None:
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise RuntimeError(f"{what}: strided tensors, got {t.layout}")
+        if t.numel() and not t.data_ptr():
+            raise RuntimeError(f"{what}: a {type(t).__name__} has no memory of its own: pass the tensor that it wraps")
+
+
 def _one_device(tensors, what: str) -> torch.device:
     devs = set(map(_device_of, tensors))
     if len(devs) != 1 or next(iter(devs)).type != "cuda":
@@ -248,9 +256,7 @@ def _listed(tensors: List[torch.Tensor], what: str):
     ptr, numel, code = _arrays(len(tensors))
     if not _tensorlist.tensors(tensors, dev.index, ptr, numel, code):
         _one_device(tensors, what)
-        for t in tensors:
-            if t.layout != torch.strided:
-                raise RuntimeError(f"{what}: strided tensors, got {t.layout}")
+        _own_memory(tensors, what)
         code = _codes(tensors, what)
         tensors = [t if t.is_contiguous() or _dense(t) else t.detach().contiguous() for t in tensors]
         ptr, numel = array("Q", map(_data_ptr, tensors)), array("Q", map(_numel, tensors))
@@ -325,20 +331,25 @@ _GLOBAL_HOOKS = (_torch_optimizer._global_optimizer_pre_hooks, _torch_optimizer.
 class _Lists:
     """A group's addresses and type codes, as the kernels' list wants them; filled anew at every step."""
 
-    def __init__(self, n: int):
-        self.p, self.g, self.p_code = _arrays(n)
+    def __init__(self, params: List[torch.Tensor]):
+        self.p, self.g, self.p_code = _arrays(len(params))
         self.g_code = array("i", self.p_code)
         self.pg, self.codes = (_addr(self.p), _addr(self.g)), (_addr(self.p_code), _addr(self.g_code))
         self.checked = (array("Q"), array("i"))            # parameters' addresses and types that were last found apart
+        self.order = [_order(p) for p in params]           # of the parameters' memory, and so of their moments
+        self.plain = all(p.is_contiguous() for p in params)
+
+
+def _order(t: torch.Tensor) -> tuple:
+    """The order of ``t``'s elements in memory: its strides, without those of axes of one element."""
+    return () if t.numel() < 2 else tuple((n, a) for n, a in zip(t.shape, t.stride()) if n != 1)
 
 
 def _in_order_of(p: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
     """``g`` with its elements in the order of ``p``'s memory."""
-    if g.layout != torch.strided:
-        raise RuntimeError(f"AdamW: strided gradients, got {g.layout}")
-    if not _dense(p):
-        raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()} has gaps or overlaps")
-    if all(a == b or n == 1 for n, a, b in zip(p.shape, p.stride(), g.stride())) or (p.is_contiguous() and g.is_contiguous()):
+    if g.shape != p.shape:
+        raise RuntimeError(f"AdamW: a gradient of shape {tuple(g.shape)} for a parameter of shape {tuple(p.shape)}")
+    if _order(g) == _order(p) and not g.is_neg():
         return g
     return torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=g.device).copy_(g)
 
@@ -387,6 +398,7 @@ class AdamW(torch.optim.Optimizer):
         try:
             _check_hyper(g)
             dev = _one_device([p for h in self.param_groups for p in h["params"]], "AdamW")
+            _own_memory(g["params"], "AdamW")
             for p in g["params"]:
                 if p.dtype not in _TYPES:
                     raise RuntimeError(f"AdamW: fp32 or bf16 parameters, got {p.dtype}")
@@ -400,7 +412,7 @@ class AdamW(torch.optim.Optimizer):
             raise
         # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
         self.moments.append(Moments([p.numel() for p in g["params"]], self.state_bits, dev))
-        self._lists.append(_Lists(len(g["params"])))
+        self._lists.append(_Lists(g["params"]))
 
     @property
     def last_grad_norm(self) -> Optional[torch.Tensor]:
@@ -432,7 +444,7 @@ class AdamW(torch.optim.Optimizer):
         counts, kept = [], []
         for k, (group, mo, ls) in enumerate(zip(self.param_groups, self.moments, self._lists)):
             n = _tensorlist.params(group["params"], mo.device.index, mo._numel, ls.p, ls.p_code, ls.g, ls.g_code)
-            if n < 0:
+            if n < 0 or not ls.plain:
                 n = self._look_closer(k, kept)
             if ls.p != ls.checked[0] or ls.p_code != ls.checked[1]:
                 self._check_memory()
@@ -465,6 +477,8 @@ class AdamW(torch.optim.Optimizer):
         for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
             if not n:
                 continue
+            if len(counts) > 1:                            # (one group: the library refuses it)
+                _check_hyper(group)
             lr, (b1, b2) = group["lr"], group["betas"]
             lr_dev = None
             if isinstance(lr, torch.Tensor):
@@ -503,6 +517,14 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError(f"AdamW: fp32 or bf16 {what}, got {sorted({str(t.dtype) for t in ts})}")
             if any(t.device != mo.device for t in ts):
                 raise RuntimeError(f"AdamW: {what} that are not on {mo.device}, where the moments are")
+            _own_memory(ts, f"AdamW: {what}")
+        for p, order in zip(params, ls.order):
+            if p.is_neg():
+                raise RuntimeError("AdamW: a parameter that is a lazily negated view")
+            # (the number of elements is known; a shape of the same order, flattened or with other axes, is the same memory)
+            if _order(p) != order and not (p.is_contiguous() and ls.plain):
+                raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()}: its memory had another "
+                                   "order when it was added, which its moments still have")
         grads = [g if g is None else _in_order_of(p, g) for p, g in zip(params, grads)]
         kept += grads
         ls.p[:] = array("Q", map(_data_ptr, params))
@@ -551,6 +573,8 @@ class AdamW(torch.optim.Optimizer):
         state = state_dict["state"]
         if any(g.get("amsgrad") for g in groups):
             raise ValueError("AdamW: no amsgrad variant")
+        if not all(g.get("decoupled_weight_decay", True) for g in groups):
+            raise ValueError("AdamW: no variant that adds the weight decay to the gradient")
         for group, saved in zip(self.param_groups, groups):
             for i, (p, key) in enumerate(zip(group["params"], saved["params"])):
                 for name in ("exp_avg", "exp_avg_sq"):
@@ -573,7 +597,7 @@ class AdamW(torch.optim.Optimizer):
             if steps:
                 mo.set_steps(steps)
             mo.write(m, v)
-            group.update({k: x for k, x in saved.items() if k != "params"})
+            group.update({k: x.clone() if isinstance(x, torch.Tensor) else x for k, x in saved.items() if k != "params"})
 
     def __getstate__(self):
         raise RuntimeError("AdamW holds device buffers: save state_dict() instead of the optimizer")

@@ -470,6 +470,86 @@ def test_layouts(bits):
     assert torch.equal(b2.moments[0].exp_avg, b.moments[0].exp_avg)
 
 
+def test_parameters_that_change_under_the_optimizer():
+    """Taken out of its group, of another order, or with a gradient of another size: refused, and nothing is written."""
+    from superresolution_amd import optim
+    w = _hash_floats(6 * 5 * 3 * 3, 1).view(6, 5, 3, 3).cuda()
+    a, b = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.clone())
+    opt = optim.AdamW([a, b], lr=1e-2)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt.step()
+    kept = b.detach().clone()
+    out = opt.param_groups[0]["params"].pop()
+    with pytest.raises(RuntimeError, match="number of elements"):
+        opt.step()
+    assert torch.equal(out, kept)
+    opt.param_groups[0]["params"].append(out)
+    opt.step()
+    assert torch.equal(a, b) and not torch.equal(b, kept)
+
+    for first, then in ((torch.contiguous_format, torch.channels_last), (torch.channels_last, torch.contiguous_format)):
+        p = torch.nn.Parameter(w.clone(memory_format=first))
+        opt = optim.AdamW([p], lr=1e-2)
+        p.grad = torch.ones_like(p)
+        opt.step()
+        p.data = p.data.contiguous(memory_format=then)
+        with pytest.raises(RuntimeError, match="another order"):
+            opt.step()
+        p.data = p.data.contiguous(memory_format=first)
+        opt.step()
+        assert opt.moments[0].steps() == [2] and torch.equal(p, a)
+
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = optim.AdamW([p], lr=1e-2)
+    p.data = torch.ones(4, device="cuda")
+    p.grad = torch.ones(4, device="cuda")
+    p.data = torch.ones(8, device="cuda")
+    with pytest.raises(RuntimeError, match="gradient of shape"):
+        opt.step()
+
+
+def test_lazily_negated_gradients():
+    from superresolution_amd import optim
+    g = _hash_floats(70, 2).cuda()
+    a, b = (torch.nn.Parameter(torch.ones(70, device="cuda")) for _ in range(2))
+    a.grad, b.grad = -g, torch._neg_view(g)
+    for p in (a, b):
+        optim.AdamW([p], lr=1e-2).step()
+    assert torch.equal(a, b)
+    assert torch.equal(optim.total_norm([a.grad]), optim.total_norm([b.grad]))
+    with pytest.raises(RuntimeError, match="negated"):
+        p = torch.nn.Parameter(torch._neg_view(torch.ones(70, device="cuda")))
+        p.grad = torch.ones_like(p)
+        optim.AdamW([p], lr=1e-2).step()
+
+
+def test_loaded_groups_are_copies():
+    from superresolution_amd import optim
+    lr = torch.tensor(1e-2, device="cuda")
+    a, b = (optim.AdamW([torch.nn.Parameter(torch.ones(8, device="cuda"))], lr=lr) for _ in range(2))
+    b.load_state_dict(a.state_dict())
+    lr.fill_(1.0)
+    assert float(b.param_groups[0]["lr"]) == float(torch.tensor(1e-2))
+    sd = a.state_dict()
+    sd["param_groups"][0]["decoupled_weight_decay"] = False
+    with pytest.raises(ValueError, match="weight decay"):
+        b.load_state_dict(sd)
+
+
+def test_a_group_with_bad_numbers_keeps_the_others_from_stepping():
+    from superresolution_amd import optim
+    a, b = (torch.nn.Parameter(torch.ones(40, device="cuda")) for _ in range(2))
+    opt = optim.AdamW([{"params": [a]}, {"params": [b]}], lr=1e-2)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    for key, bad in (("lr", -1.0), ("betas", (0.9, 1.0)), ("eps", float("nan")), ("weight_decay", -1.0)):
+        good = opt.param_groups[1][key]
+        opt.param_groups[1][key] = bad
+        with pytest.raises(ValueError, match="Invalid"):
+            opt.step()
+        opt.param_groups[1][key] = good
+    assert torch.equal(a, torch.ones_like(a)) and opt.moments[0].steps() == [0]
+
+
 def test_refusals_on_the_device():
     from superresolution_amd import optim
     t = torch.zeros(64, device="cuda")

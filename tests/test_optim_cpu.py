@@ -201,3 +201,33 @@ def test_moments_update_refuses_other_lists(bits):
         lists[k] = array("I", [0, 0]) if k < 2 else array("h", [0, 0])
         with pytest.raises(TypeError, match="type codes"):
             mo.update(*lists, args, 0)
+
+
+def test_a_shorter_parameter_list_wants_a_closer_look():
+    """The arrays still hold the addresses of a parameter that was taken out of its group: not to be launched with."""
+    from array import array
+    from superresolution_amd import _tensorlist
+    q, i = (lambda n: array("Q", [7] * n)), (lambda n: array("i", [0] * n))
+    assert _tensorlist.params([], 0, q(1), q(1), i(1), q(1), i(1)) == -1
+    assert _tensorlist.params([], 0, q(0), q(0), i(0), q(0), i(0)) == 0
+
+
+def _wrapper(n, dtype=torch.float32):
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls):
+            return torch.Tensor._make_wrapper_subclass(cls, (n,), dtype=dtype, device="cuda:0")
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError(str(func))
+
+    return Wrapper()
+
+
+def test_tensors_without_memory_are_refused():
+    """A subclass that wraps another tensor has address 0, which stands for a tensor that is left out."""
+    from superresolution_amd import optim
+    for f in (optim.total_norm, lambda ts: optim.AdamW(ts)):
+        with pytest.raises(RuntimeError, match="no memory of its own"):
+            f([_wrapper(5)])
