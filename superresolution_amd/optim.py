@@ -367,7 +367,8 @@ class AdamW(torch.optim.Optimizer):
     ``seed``            of the stochastic rounding, which depends on it, the step and the element only.
 
     A bf16 parameter is rounded stochastically.  ``lr`` may be a 0-dim fp32 tensor on the parameters' device: a captured step
-    then follows it.  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
+    then follows it.  Parameters keep the memory order that they were added with (``to(memory_format=...)`` comes before the
+    optimizer).  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
     optimizer have to stay.  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
     gradient does not happen.  ``state_dict`` has the layout of ``torch.optim.AdamW`` with fp32 moments, whatever
     ``state_bits``: checkpoints move between the two, and between 8 and 32 bits (``state`` stays empty: ``moments`` has one

@@ -332,6 +332,18 @@ def test_vanishing_learning_rates_and_zero_gradients(bits, lr):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_vanishing_eps_and_zero_gradients(bits):
+    """0 / eps is 0 for the smallest eps too."""
+    from superresolution_amd import optim
+    p = torch.nn.Parameter(torch.ones(100, device="cuda"))
+    opt = optim.AdamW([p], lr=0.5, eps=1e-42, weight_decay=0.0, state_bits=bits)
+    for _ in range(2):
+        p.grad = torch.zeros_like(p)
+        opt.step()
+    assert torch.equal(p, torch.ones_like(p))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("max_norm", [0.5, 1e6])
 def test_clip_inside_the_step(bits, max_norm):
     from superresolution_amd import optim
