@@ -117,13 +117,14 @@ class Moments:
     def __init__(self, numels: List[int], bits: int, device: torch.device):
         if bits not in (8, 32):
             raise ValueError(f"moments of {bits} bits: 8 or 32")
-        self.numels, self.bits, self.device = list(numels), bits, device
+        self.numels, self.bits = list(numels), bits
         sizes = [_up(n, BLOCK) for n in numels]
         self.offsets = [0, *accumulate(sizes)][:-1]
         self.total = sum(sizes)
         counters = [-(-n // CHUNK) for n in numels]
         self.counter0 = [0, *accumulate(counters)]
         self.step = torch.zeros(self.counter0[-1], dtype=torch.int32, device=device)
+        self.device = self.step.device                     # (with its index)
         if bits == 32:
             self.exp_avg = torch.zeros(self.total, dtype=torch.float32, device=device)
             self.exp_avg_sq = torch.zeros(self.total, dtype=torch.float32, device=device)
@@ -171,6 +172,10 @@ class Moments:
 
     def write(self, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor) -> None:
         """Takes fp32 buffers in the padded layout (the padding has to be zero)."""
+        for t in (exp_avg, exp_avg_sq):
+            if t.dtype != torch.float32 or t.shape != (self.total,) or t.device != self.device or not t.is_contiguous():
+                raise RuntimeError(f"Moments.write: flat contiguous fp32 buffers of {self.total} elements on {self.device}, got "
+                                   f"{tuple(t.shape)} {t.dtype} on {t.device}")
         if self.bits == 32:
             self.exp_avg.copy_(exp_avg)
             self.exp_avg_sq.copy_(exp_avg_sq)

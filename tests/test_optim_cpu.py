@@ -231,3 +231,14 @@ def test_tensors_without_memory_are_refused():
     for f in (optim.total_norm, lambda ts: optim.AdamW(ts)):
         with pytest.raises(RuntimeError, match="no memory of its own"):
             f([_wrapper(5)])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_write_refuses_other_buffers(bits):
+    from superresolution_amd import optim
+    mo = optim.Moments([5, 40], bits, torch.device("cpu"))
+    good = torch.zeros(mo.total)
+    for bad in (torch.zeros(mo.total + 32), torch.zeros(1), good.double(), torch.zeros(2 * mo.total)[::2], good.to("meta")):
+        for pair in ((bad, good), (good, bad)):
+            with pytest.raises(RuntimeError, match="Moments.write"):
+                mo.write(*pair)
