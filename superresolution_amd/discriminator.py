@@ -23,7 +23,7 @@ from typing import Dict, Optional, Tuple
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _lib, versions
 
 
 class DiscBlock(nn.Module):
@@ -87,11 +87,12 @@ class Discriminator(nn.Module):
 
     # ---- HIP handle / weights ----------------------------------------------------------
     def _signature(self) -> Tuple:
-        return tuple((t.data_ptr(), t._version) for t in self.state_dict(keep_vars=True).values())
+        return tuple(map(versions.tag, self.state_dict(keep_vars=True).values()))
 
     def _handle(self, idx: int) -> int:
         L = _lib.lib()
         if idx not in self._handles:
+            versions.refuse_capture("Discriminator", idx)
             cfg = _lib.srdisc_config(self.in_ch, self.base_ch)
             h = ctypes.c_void_p()
             with torch.cuda.device(idx):
@@ -100,6 +101,7 @@ class Discriminator(nn.Module):
         h = self._handles[idx]
         sig = self._signature()
         if self._weights_sig.get(idx) != sig:
+            versions.refuse_capture("Discriminator", idx)
             keep = []
             for key, t in self.state_dict().items():
                 c = t.detach().to(device="cpu", dtype=torch.float32).contiguous()

@@ -21,7 +21,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, versions
 from .training import FlatAdamW, PretrainStep, Workspace, _timed, allreduce_mean, conv_precision, packed_weights, pixel_loss_grad, resolve_precision
 
 SLOPE = 0.2                                  # nn.LeakyReLU(0.2), Discriminator.py:10,24,36
@@ -99,7 +99,7 @@ class DiscriminatorGrad:
         raw kernels) need ``invalidate_packs()``."""
         p = conv.weight
         bf16 = bf16 and mode in (0, 1, 4)
-        key, tag = (id(conv), mode, bf16), (p._version, p.data_ptr())
+        key, tag = (id(conv), mode, bf16), versions.tag(p)
         hit = self._packs.get(key)
         if hit is not None and hit[0] == tag:
             return hit[1]

@@ -26,7 +26,7 @@ from typing import Dict, Optional, Tuple
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _lib, versions
 
 
 class _Container(nn.Module):
@@ -98,13 +98,13 @@ class Generator(nn.Module):
     def _signature(self) -> Tuple:
         """(parameters, buffers): the train-mode forward reads no BatchNorm running statistics, so its own
         updates of those buffers must not force a re-upload before the next train-mode call."""
-        return (tuple((t.data_ptr(), t._version) for t in self.parameters()),
-                tuple((t.data_ptr(), t._version) for t in self.buffers()))
+        return tuple(map(versions.tag, self.parameters())), tuple(map(versions.tag, self.buffers()))
 
     def _handle(self, device: torch.device, train: bool = False) -> int:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         L = _lib.lib()
         if idx not in self._handles:
+            versions.refuse_capture("Generator", idx)
             cfg = _lib.srgen_config(self.num_blocks, self.in_ch, self.base_ch)
             h = ctypes.c_void_p()
             with torch.cuda.device(idx):
@@ -114,6 +114,7 @@ class Generator(nn.Module):
         sig = self._signature()
         have = self._weights_sig.get(idx)
         if have != sig and not (train and have is not None and have[0] == sig[0]):
+            versions.refuse_capture("Generator", idx)
             self._upload(h, idx)
             self._weights_sig[idx] = sig
         return h

@@ -26,7 +26,7 @@ from typing import List, Optional, Tuple
 import torch
 from torch.optim import optimizer as _torch_optimizer
 
-from . import _lib
+from . import _lib, versions
 
 
 class _NotBuilt:
@@ -49,6 +49,7 @@ BLOCK = 32            # SRGEN_OPT_BLOCK: elements that share one scale (8-bit mo
 CHUNK = 4096          # SRGEN_OPT_CHUNK: elements of one step counter
 
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(dev).cuda_stream without the object
+_capturing = torch.cuda.is_current_stream_capturing
 _CODE = {torch.float32: _lib.SRGEN_F32, torch.bfloat16: _lib.SRGEN_BF16, torch.float16: _lib.SRGEN_F16}
 _TYPES = frozenset((torch.float32, torch.bfloat16))                  # of parameters and their gradients
 _dtype_of, _device_of = attrgetter("dtype"), attrgetter("device")
@@ -374,7 +375,8 @@ class AdamW(torch.optim.Optimizer):
     A bf16 parameter is rounded stochastically.  ``lr`` may be a 0-dim fp32 tensor on the parameters' device: a captured step
     then follows it.  Parameters keep the memory order that they were added with (``to(memory_format=...)`` comes before the
     optimizer).  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
-    optimizer have to stay.  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
+    optimizer have to stay.  While it does, ``Generator`` and ``Discriminator`` take its parameters for changed at every use (a replay
+    raises no version counter, ``versions``).  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
     gradient does not happen.  ``state_dict`` has the layout of ``torch.optim.AdamW`` with fp32 moments, whatever
     ``state_bits``: checkpoints move between the two, and between 8 and 32 bits (``state`` stays empty: ``moments`` has one
     ``Moments`` for each group).
@@ -505,6 +507,9 @@ class AdamW(torch.optim.Optimizer):
                 # the kernel wrote behind torch's back: the version counters are what the Generator / Discriminator mirrors
                 # watch to upload their weights again
                 _tensorlist.bump(group["params"], ls.g)
+            if _capturing():                               # (its replays will write them, and raise no counter)
+                for group, _, ls, _ in calls:
+                    versions.note_captured((p for p, g in zip(group["params"], ls.g) if g), self)
         return loss
 
     _step_with_hooks = torch.optim.Optimizer.profile_hook_step(_step)

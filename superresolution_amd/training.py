@@ -19,7 +19,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, versions
 from .optim import Moments
 
 WINO_FLOATS = 16 * 96 * 96           # Winograd weight image of one 96 -> 96 conv
@@ -569,6 +569,8 @@ class FlatAdamW(torch.optim.Optimizer):
                 fp32 = array("i", [_lib.SRGEN_F32])
                 self.moments.update(array("Q", [self.flat.data_ptr()]), array("Q", [self.flat_grad.data_ptr()]), fp32, fp32, args,
                                     _stream(self.flat))
+                if torch.cuda.is_current_stream_capturing():             # (replays raise no version counter)
+                    versions.note_captured(self.params, self)
             torch.autograd.graph.increment_version(self.params)
             return
         with torch.cuda.device(self.flat.device):

@@ -1,0 +1,98 @@
+"""GPU: optimizer steps that are captured and replayed, beside the package's own modules, eager steps and loaded checkpoints;
+refused steps; learning rates of zero."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import optim_ref as R
+from test_gpu_optim import _check, _f64, _hash_floats
+
+pytestmark = pytest.mark.gpu
+
+
+def _capture(f):
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        f()
+    torch.cuda.current_stream().wait_stream(side)
+    return graph
+
+
+def _give_gradients(module, scale=1e-2):
+    for i, p in enumerate(module.parameters()):
+        p.grad = (_hash_floats(p.numel(), 900 + i, scale)).view(p.shape).cuda()
+
+
+def _copy_of(module):
+    other = type(module)().cuda().train(module.training)
+    other.load_state_dict(module.state_dict())
+    return other
+
+
+# ---- the package's modules behind a captured step ----------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["list 32", "list 8", "flat 8"])
+def test_generator_after_replays_of_a_captured_step(which):
+    """eval() forwards with the weights that the last replay left, as a module that was given these weights computes."""
+    from superresolution_amd import Generator, optim
+    from superresolution_amd.training import FlatAdamW
+    torch.manual_seed(0)
+    gen = Generator().cuda().eval()
+    x = torch.rand(1, 3, 64, 64, device="cuda")
+    if which == "flat 8":
+        opt = FlatAdamW(gen.parameters(), lr=1e-3, state_bits=8)
+        opt.flat_grad.copy_(_hash_floats(opt.flat.numel(), 3, 1e-2))
+    else:
+        opt = optim.AdamW(gen.parameters(), lr=1e-3, state_bits=int(which[-2:]))
+        _give_gradients(gen)
+    with torch.no_grad():
+        last = gen(x)
+        graph = _capture(opt.step)
+        for k in range(4):
+            graph.replay()
+            y = gen(x)
+            assert not torch.equal(y, last), k
+            assert torch.equal(y, _copy_of(gen)(x)), k
+            last = y
+        opt.step()                                                     # an eager step between replays
+        assert torch.equal(gen(x), _copy_of(gen)(x))
+        graph.replay()
+        assert torch.equal(gen(x), _copy_of(gen)(x))
+
+
+def test_discriminator_after_replays_of_a_captured_step():
+    """Logits without a graph, and logits and gradients of the training route, with the weights of the last replay."""
+    from superresolution_amd import Discriminator, optim
+    torch.manual_seed(0)
+    disc = Discriminator().cuda().train()
+    x = torch.rand(2, 3, 37, 53, device="cuda")
+
+    def all_of(d):
+        with torch.no_grad():
+            values = d(x)
+        logits = d(x)
+        return [values, logits.detach(), *torch.autograd.grad(logits.square().sum(), list(d.parameters()))]
+    opt = optim.AdamW(disc.parameters(), lr=1e-3)
+    _give_gradients(disc)
+    last = all_of(disc)
+    graph = _capture(opt.step)
+    for k in range(4):
+        graph.replay()
+        got, want = all_of(disc), all_of(_copy_of(disc))
+        assert not torch.equal(got[0], last[0]) and not torch.equal(got[1], last[1]), k
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+        last = got
+
+
+def test_a_forward_that_would_upload_weights_is_refused_in_a_capture():
+    """The upload goes through the host, which a graph does not replay.  The refusal comes before anything is recorded."""
+    from superresolution_amd import Discriminator, Generator
+    for module, x in ((Generator().cuda().eval(), torch.rand(1, 3, 64, 64, device="cuda")), (Discriminator().cuda(), torch.rand(1, 3, 20, 20, device="cuda"))):
+        with torch.no_grad():
+            module(x)
+            next(module.parameters()).mul_(1.5)
+            side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+            with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+                with pytest.raises(RuntimeError, match="capture"):
+                    module(x)
+            assert torch.equal(module(x), _copy_of(module)(x))

@@ -1,0 +1,67 @@
+"""CPU: what an optimizer over a list of tensors does around its steps -- groups that fail to be added, checkpoints and their
+hooks, parameters that change under it -- with the moments in host memory (nothing is launched), and the tags by which the modules
+know that weights have changed."""
+import gc
+
+import numpy as np
+import pytest
+import torch
+
+
+@pytest.fixture
+def optim(monkeypatch):
+    """The module, with the check for a ROCm device put aside."""
+    from superresolution_amd import optim
+    monkeypatch.setattr(optim, "_one_device", lambda ts, what: torch.device("cpu"))
+    return optim
+
+
+def _filled(optim, params, **kw):
+    """An optimizer that has taken three steps, its moments told apart by element."""
+    opt = optim.AdamW(params, lr=1e-2, **kw)
+    for mo in opt.moments:
+        mo.set_steps([3] * len(mo.numels))
+        mo.exp_avg.copy_(torch.arange(mo.total) + 1.0)
+        mo.exp_avg_sq.copy_(torch.arange(mo.total) + 0.5)
+    return opt
+
+
+def test_tags_of_parameters_that_a_graph_writes():
+    """A tag is the same again while nothing has written the tensor; never, where a replay may have, unseen by the host."""
+    from superresolution_amd import versions
+
+    class Owner:
+        pass
+    a, b = torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(3))
+    assert versions.tag(a) == versions.tag(a) != versions.tag(b)
+    was = versions.tag(a)
+    with torch.no_grad():
+        a.mul_(2.0)
+    assert versions.tag(a) != was
+    one, two = Owner(), Owner()
+    versions.note_captured([a], one)
+    versions.note_captured([a], two)
+    assert versions.tag(a) != versions.tag(a) and versions.tag(b) == versions.tag(b)
+    del one
+    gc.collect()
+    assert versions.tag(a) != versions.tag(a)
+    last = versions.tag(a)
+    del two                                                              # no graph may be replayed after its optimizer
+    gc.collect()
+    assert versions.tag(a) == versions.tag(a) != last
+
+
+def test_modules_go_by_the_tags():
+    """The signatures by which Generator and Discriminator know that their uploaded weights are still the parameters'."""
+    from superresolution_amd import Discriminator, Generator, versions
+
+    class Owner:
+        pass
+    for module in (Generator(), Discriminator()):
+        assert module._signature() == module._signature()
+        owner = Owner()
+        versions.note_captured(list(module.parameters())[-1:], owner)
+        assert module._signature() != module._signature()
+        del owner
+        gc.collect()
+        assert module._signature() == module._signature()
