@@ -96,12 +96,14 @@ class DiscriminatorGrad:
         discriminator is updated every third iteration only (config.py:21), and a generator half-step packs the same
         weights its discriminator half-step just used.  A change is an in-place update (the version counter every torch
         optimizer and FlatAdamW bump) or a new storage.  Writes that bypass the version counter (``p.data.copy_(...)``,
-        raw kernels) need ``invalidate_packs()``."""
+        raw kernels) need ``invalidate_packs()``.  A forward or backward that is being captured makes its own images: kept
+        ones would be those of the capture at every replay, and ones made inside the graph hold nothing before it runs."""
         p = conv.weight
         bf16 = bf16 and mode in (0, 1, 4)
         key, tag = (id(conv), mode, bf16), versions.tag(p)
+        capturing = torch.cuda.is_current_stream_capturing()
         hit = self._packs.get(key)
-        if hit is not None and hit[0] == tag:
+        if hit is not None and hit[0] == tag and not capturing:
             return hit[1]
         w = p.detach().contiguous()
         cout, cin = w.shape[0], w.shape[1]
@@ -110,7 +112,8 @@ class DiscriminatorGrad:
         fn = _lib.lib().srdisc_pack_bf16 if bf16 else _lib.lib().srdisc_pack
         with torch.cuda.device(w.device):
             _lib.check(fn(w.data_ptr(), cin, cout, mode, out.data_ptr(), _stream(w)))
-        self._packs[key] = (tag, out)
+        if not capturing:
+            self._packs[key] = (tag, out)
         return out
 
     def invalidate_packs(self) -> None:

@@ -84,6 +84,28 @@ def test_discriminator_after_replays_of_a_captured_step():
         last = got
 
 
+def test_captured_discriminator_forward_follows_the_weights():
+    """The kernel-side weight images are made inside the graph, not taken from an earlier call."""
+    from superresolution_amd import Discriminator
+    from superresolution_amd.gan_training import DiscriminatorGrad
+    from superresolution_amd.training import Workspace
+    torch.manual_seed(0)
+    disc = Discriminator().cuda()
+    x = torch.rand(2, 3, 37, 53, device="cuda")
+    dg, out = DiscriminatorGrad(disc, Workspace(x.device)), []
+    first = dg.forward(x)[0]
+    graph = _capture(lambda: out.append(dg.forward(x)[0]))
+    for k in range(4):
+        with torch.no_grad():
+            for p in disc.parameters():
+                p.mul_(1.1)
+        graph.replay()
+        got = out[0].clone()
+        want = dg.forward(x)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and not torch.equal(got, first), k
+
+
 def test_a_forward_that_would_upload_weights_is_refused_in_a_capture():
     """The upload goes through the host, which a graph does not replay.  The refusal comes before anything is recorded."""
     from superresolution_amd import Discriminator, Generator
