@@ -485,8 +485,6 @@ class AdamW(torch.optim.Optimizer):
         for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
             if not n:
                 continue
-            if len(counts) > 1:                            # (one group: the library refuses it)
-                _check_hyper(group)
             lr, (b1, b2) = group["lr"], group["betas"]
             lr_dev = None
             if isinstance(lr, torch.Tensor):
@@ -496,6 +494,8 @@ class AdamW(torch.optim.Optimizer):
                     lr_dev, lr = lr.data_ptr(), 0.0
                 else:
                     lr = float(lr)
+            if len(counts) > 1:                            # (one group: the library refuses it)
+                _check_hyper({**group, "lr": lr})
             calls.append((group, mo, ls, _lib.srgen_adamw_args(
                 lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, mul, None if div is None else div.data_ptr(),
                 None if found is None else found.data_ptr(), out, scratch, mo.norm_bytes, self.max_grad_norm or 0.0, self.seed,

@@ -118,3 +118,16 @@ def test_a_forward_that_would_upload_weights_is_refused_in_a_capture():
                 with pytest.raises(RuntimeError, match="capture"):
                     module(x)
             assert torch.equal(module(x), _copy_of(module)(x))
+
+
+# ---- the clipped step's norm -------------------------------------------------------------------------------------------
+def test_a_negative_learning_rate_on_the_host_keeps_every_group_from_stepping():
+    from superresolution_amd import optim
+    a, b = (torch.nn.Parameter(torch.ones(40, device="cuda")) for _ in range(2))
+    opt = optim.AdamW([dict(params=[a]), dict(params=[b])], lr=1e-2)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    for bad in (-1.0, float("nan")):
+        opt.param_groups[1]["lr"] = torch.tensor(bad)
+        with pytest.raises((RuntimeError, ValueError), match="lr|learning rate"):
+            opt.step()
+    assert torch.equal(a, torch.ones_like(a)) and opt.moments[0].steps() == [0]
