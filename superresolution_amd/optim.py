@@ -464,23 +464,9 @@ class AdamW(torch.optim.Optimizer):
         for t in (div, found):
             if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != 1):
                 raise RuntimeError(f"AdamW: grad_scale and found_inf are fp32 scalars on {dev}")
-        mul = out = scratch = None
-        if self.max_grad_norm is not None:
-            if div is not None:
-                raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
-                                   "scaler.step(optimizer)")
-            if len(counts) == 1:                           # norm and step in one call
-                mo = self.moments[0]
-                buf = torch.empty(mo.norm_bytes // 4 + 2, dtype=torch.float32, device=dev)
-                scratch = buf.data_ptr()
-                out = scratch + mo.norm_bytes
-                self._norm_coef = buf
-            else:
-                g, numel, code = array("Q"), array("Q"), array("i")
-                for mo, ls in zip(self.moments, self._lists):
-                    g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
-                self._norm_coef = _norm_coef(dev, g, numel, code, self.max_grad_norm)
-                mul = self._norm_coef.data_ptr() + 4 * (self._norm_coef.numel() - 1)
+        if self.max_grad_norm is not None and div is not None:
+            raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
+                               "scaler.step(optimizer)")
         calls = []                                         # (all of them before the first: no group steps if another is refused)
         for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
             if not n:
@@ -497,9 +483,23 @@ class AdamW(torch.optim.Optimizer):
             if len(counts) > 1:                            # (one group: the library refuses it)
                 _check_hyper({**group, "lr": lr})
             calls.append((group, mo, ls, _lib.srgen_adamw_args(
-                lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, mul, None if div is None else div.data_ptr(),
-                None if found is None else found.data_ptr(), out, scratch, mo.norm_bytes, self.max_grad_norm or 0.0, self.seed,
+                lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, None, None if div is None else div.data_ptr(),
+                None if found is None else found.data_ptr(), None, None, mo.norm_bytes, self.max_grad_norm or 0.0, self.seed,
                 1 if group["maximize"] else 0)))
+        norm_coef = None
+        if self.max_grad_norm is not None:
+            if len(counts) == 1:                           # norm and step in one call
+                mo, args = self.moments[0], calls[0][3]
+                norm_coef = torch.empty(mo.norm_bytes // 4 + 2, dtype=torch.float32, device=dev)
+                args.norm_scratch = norm_coef.data_ptr()
+                args.norm_coef2 = args.norm_scratch + mo.norm_bytes
+            else:
+                g, numel, code = array("Q"), array("Q"), array("i")
+                for mo, ls in zip(self.moments, self._lists):
+                    g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
+                norm_coef = _norm_coef(dev, g, numel, code, self.max_grad_norm)
+                for *_, args in calls:
+                    args.grad_mul = norm_coef.data_ptr() + 4 * (norm_coef.numel() - 1)
         with _on(dev):
             stream = _stream(dev)
             for group, mo, ls, args in calls:
@@ -510,6 +510,8 @@ class AdamW(torch.optim.Optimizer):
             if _capturing():                               # (its replays will write them, and raise no counter)
                 for group, _, ls, _ in calls:
                     versions.note_captured((p for p, g in zip(group["params"], ls.g) if g), self)
+        if norm_coef is not None:                          # (a refused step leaves the last one's)
+            self._norm_coef = norm_coef
         return loss
 
     _step_with_hooks = torch.optim.Optimizer.profile_hook_step(_step)

@@ -121,6 +121,35 @@ def test_a_forward_that_would_upload_weights_is_refused_in_a_capture():
 
 
 # ---- the clipped step's norm -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("groups", [1, 2])
+def test_a_refused_step_leaves_the_last_norm(groups):
+    from superresolution_amd import optim
+    ps = [torch.nn.Parameter(_hash_floats(n, n).cuda()) for n in (500, 77)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = optim.AdamW(ps if groups == 1 else [dict(params=[p]) for p in ps], lr=1e-3, max_grad_norm=0.3)
+    bad = (("lr", -1.0), ("betas", (0.9, 1.0)), ("lr", torch.tensor(1e-3, dtype=torch.float64, device="cuda")), ("lr", torch.tensor(-1.0)))
+
+    def refused():
+        for key, value in bad:
+            good = opt.param_groups[-1][key]
+            opt.param_groups[-1][key] = value
+            torch.full((4096,), -5.0, device="cuda")
+            with pytest.raises((RuntimeError, ValueError)):
+                opt.step()
+            opt.param_groups[-1][key] = good
+    refused()
+    assert opt.last_grad_norm is None
+    opt.step()
+    want = optim.total_norm([p.grad for p in ps])
+    kept = [p.detach().clone() for p in ps]
+    for p in ps:
+        p.grad.mul_(3.0)
+    refused()
+    assert torch.equal(opt.last_grad_norm, want)
+    assert all(torch.equal(a, p) for a, p in zip(kept, ps)) and [mo.steps()[0] for mo in opt.moments] == [1] * groups
+
+
 def test_a_negative_learning_rate_on_the_host_keeps_every_group_from_stepping():
     from superresolution_amd import optim
     a, b = (torch.nn.Parameter(torch.ones(40, device="cuda")) for _ in range(2))
