@@ -269,14 +269,14 @@ def _listed(tensors: List[torch.Tensor], what: str):
     return dev, tensors, ptr, numel, code
 
 
-def _norm_coef(dev: torch.device, ptr: array, numel: array, code: array, max_norm: float) -> torch.Tensor:
-    """A device buffer that ends with {norm, clip coefficient}; address 0: left out."""
+def _norm_coef(dev: torch.device, ptr: array, numel: array, code: array, max_norm: float, out: Optional[int] = None) -> torch.Tensor:
+    """A device buffer that ends with {norm, clip coefficient}, or they go to the address ``out``; tensor address 0: left out."""
     L, need = _lib.lib(), ctypes.c_size_t()
     _lib.check(L.srgen_total_norm_scratch_bytes(len(ptr), _addr(numel), need))
     words = need.value // 4
     buf = torch.empty(words + 2, dtype=torch.float32, device=dev)              # partial sums, then {norm, coefficient}
     with _on(dev):
-        _lib.check(L.srgen_total_norm(len(ptr), _addr(ptr), _addr(numel), _addr(code), max_norm, buf.data_ptr() + need.value, buf.data_ptr(),
+        _lib.check(L.srgen_total_norm(len(ptr), _addr(ptr), _addr(numel), _addr(code), max_norm, out or buf.data_ptr() + need.value, buf.data_ptr(),
                                       need.value, _stream(dev)))
     return buf
 
@@ -395,7 +395,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"max_grad_norm={max_grad_norm}: positive, or None")
         self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFF
         self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
-        self._norm_coef: Optional[torch.Tensor] = None     # ends with {norm, clip coefficient} of the last step
+        self._norm_coef: Optional[torch.Tensor] = None     # ends with {norm, clip coefficient} of the last eager step
+        # the same of every step from the first captured one on: a replay writes where the capture did, and the host does not see it
+        self._norm_fixed: Optional[torch.Tensor] = None
+        self._captured = False                             # a step has been captured
         self.moments: List[Moments] = []
         self._lists: List[_Lists] = []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
@@ -421,11 +424,18 @@ class AdamW(torch.optim.Optimizer):
         # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
         self.moments.append(Moments([p.numel() for p in g["params"]], self.state_bits, dev))
         self._lists.append(_Lists(g["params"]))
+        if self.max_grad_norm is not None and self._norm_fixed is None:
+            self._norm_fixed = torch.full((2,), -1.0, dtype=torch.float32, device=dev)      # (-1: nothing yet)
 
     @property
     def last_grad_norm(self) -> Optional[torch.Tensor]:
-        """The gradients' total norm at the last step that clipped, before clipping (0-dim device tensor)."""
-        return None if self._norm_coef is None else self._norm_coef[-2]
+        """The gradients' total norm at the last step that clipped, eager or replayed, before clipping (0-dim device tensor; NaN
+        where a step has been captured and none has run)."""
+        if not self._captured or self._norm_fixed is None:
+            return None if self._norm_coef is None else self._norm_coef[-2]
+        # (a new tensor: the next step writes the buffer)
+        norm = self._norm_fixed[0]
+        return norm.masked_fill(norm < 0, float("nan")) if self._norm_coef is None else torch.where(norm < 0, self._norm_coef[-2], norm)
 
     # -- one step -----------------------------------------------------------------------------------------------------
     def step(self, closure=None):
@@ -486,31 +496,34 @@ class AdamW(torch.optim.Optimizer):
                 lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, None, None if div is None else div.data_ptr(),
                 None if found is None else found.data_ptr(), None, None, mo.norm_bytes, self.max_grad_norm or 0.0, self.seed,
                 1 if group["maximize"] else 0)))
-        norm_coef = None
-        if self.max_grad_norm is not None:
-            if len(counts) == 1:                           # norm and step in one call
-                mo, args = self.moments[0], calls[0][3]
-                norm_coef = torch.empty(mo.norm_bytes // 4 + 2, dtype=torch.float32, device=dev)
-                args.norm_scratch = norm_coef.data_ptr()
-                args.norm_coef2 = args.norm_scratch + mo.norm_bytes
-            else:
-                g, numel, code = array("Q"), array("Q"), array("i")
-                for mo, ls in zip(self.moments, self._lists):
-                    g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
-                norm_coef = _norm_coef(dev, g, numel, code, self.max_grad_norm)
-                for *_, args in calls:
-                    args.grad_mul = norm_coef.data_ptr() + 4 * (norm_coef.numel() - 1)
         with _on(dev):
-            stream = _stream(dev)
+            stream, capturing = _stream(dev), _capturing()
+            norm_coef = fixed = None
+            if self.max_grad_norm is not None:
+                if capturing or self._captured:
+                    fixed = self._norm_fixed.data_ptr()
+                if len(counts) == 1:                       # norm and step in one call
+                    mo, args = self.moments[0], calls[0][3]
+                    norm_coef = torch.empty(mo.norm_bytes // 4 + 2, dtype=torch.float32, device=dev)
+                    args.norm_scratch = norm_coef.data_ptr()
+                    args.norm_coef2 = fixed or args.norm_scratch + mo.norm_bytes
+                else:
+                    g, numel, code = array("Q"), array("Q"), array("i")
+                    for mo, ls in zip(self.moments, self._lists):
+                        g, numel, code = g + ls.g, numel + mo._numel, code + ls.g_code
+                    norm_coef = _norm_coef(dev, g, numel, code, self.max_grad_norm, fixed)
+                    for *_, args in calls:
+                        args.grad_mul = (fixed or norm_coef.data_ptr() + 4 * (norm_coef.numel() - 2)) + 4
             for group, mo, ls, args in calls:
                 mo._update(ls.pg, ls.codes, args, stream)
                 # the kernel wrote behind torch's back: the version counters are what the Generator / Discriminator mirrors
                 # watch to upload their weights again
                 _tensorlist.bump(group["params"], ls.g)
-            if _capturing():                               # (its replays will write them, and raise no counter)
+            if capturing:                                  # (its replays will write them, and raise no counter)
+                self._captured = True
                 for group, _, ls, _ in calls:
                     versions.note_captured((p for p, g in zip(group["params"], ls.g) if g), self)
-        if norm_coef is not None:                          # (a refused step leaves the last one's)
+        if norm_coef is not None and not fixed:            # (a refused step leaves the last one's)
             self._norm_coef = norm_coef
         return loss
 

@@ -122,6 +122,45 @@ def test_a_forward_that_would_upload_weights_is_refused_in_a_capture():
 
 # ---- the clipped step's norm -------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("groups", [1, 2])
+def test_last_grad_norm_between_eager_steps_and_replays(groups):
+    """The norm of the step that was last executed, replayed or not; values read earlier stay what they were."""
+    from superresolution_amd import optim
+    ps = [torch.nn.Parameter(_hash_floats(n, n).cuda()) for n in (5000, 77)]
+    for i, p in enumerate(ps):
+        p.grad = _hash_floats(p.numel(), 30 + i, 1e-2).cuda()
+    opt = optim.AdamW(ps if groups == 1 else [dict(params=[p]) for p in ps], lr=1e-3, max_grad_norm=0.3)
+    assert opt.last_grad_norm is None
+
+    def scaled():
+        for p in ps:
+            p.grad.mul_(1.5)
+        return optim.total_norm([p.grad for p in ps])
+    seen = [(scaled(), opt.step(), opt.last_grad_norm)]
+    inside = []
+    graph = _capture(lambda: (opt.step(), inside.append(opt.last_grad_norm)))
+    assert torch.equal(opt.last_grad_norm, seen[0][0])                # nothing has been executed since
+    for kind in ("replay", "replay", "eager", "replay", "eager", "eager", "replay"):
+        want = scaled()
+        (graph.replay if kind == "replay" else opt.step)()
+        torch.full((4096,), -5.0, device="cuda")
+        seen.append((want, None, opt.last_grad_norm))
+        if kind == "replay":
+            assert torch.equal(inside[0], want)
+    assert all(torch.equal(want, got) for want, _, got in seen)
+
+
+def test_last_grad_norm_of_a_captured_first_step():
+    from superresolution_amd import optim
+    p = torch.nn.Parameter(_hash_floats(500, 1).cuda())
+    p.grad = _hash_floats(500, 2).cuda()
+    opt = optim.AdamW([p], lr=1e-3, max_grad_norm=0.3)
+    graph = _capture(opt.step)
+    assert torch.isnan(opt.last_grad_norm)                              # no step yet
+    graph.replay()
+    assert torch.equal(opt.last_grad_norm, optim.total_norm([p.grad]))
+
+
+@pytest.mark.parametrize("groups", [1, 2])
 def test_a_refused_step_leaves_the_last_norm(groups):
     from superresolution_amd import optim
     ps = [torch.nn.Parameter(_hash_floats(n, n).cuda()) for n in (500, 77)]
