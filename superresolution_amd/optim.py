@@ -373,7 +373,7 @@ class AdamW(torch.optim.Optimizer):
     ``seed``            of the stochastic rounding, which depends on it, the step and the element only.
 
     A bf16 parameter is rounded stochastically.  ``lr`` may be a 0-dim fp32 tensor on the parameters' device: a captured step
-    then follows it.  Parameters keep the memory order that they were added with (``to(memory_format=...)`` comes before the
+    then follows it, and ``load_state_dict`` writes into it (before a capture it makes a new one, as torch does).  Parameters keep the memory order that they were added with (``to(memory_format=...)`` comes before the
     optimizer).  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
     optimizer have to stay.  While it does, ``Generator`` and ``Discriminator`` take its parameters for changed at every use (a replay
     raises no version counter, ``versions``).  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
@@ -623,7 +623,15 @@ class AdamW(torch.optim.Optimizer):
             if steps:
                 mo.set_steps(steps)
             mo.write(m, v)
-            group.update({k: x.clone() if isinstance(x, torch.Tensor) else x for k, x in saved.items() if k != "params"})
+            lr = self._loaded_lr(group["lr"], saved.get("lr", group["lr"]))
+            group.update({k: x.clone() if isinstance(x, torch.Tensor) else x for k, x in saved.items() if k not in ("params", "lr")}, lr=lr)
+
+    def _loaded_lr(self, lr, saved):
+        """What a group's learning rate becomes: a scalar on the device stays one, and the very one that a captured step reads."""
+        if isinstance(lr, torch.Tensor) and lr.is_cuda:
+            saved = torch.as_tensor(saved).reshape(lr.shape)
+            return lr.copy_(saved) if self._captured else torch.empty_like(lr).copy_(saved)
+        return saved.clone() if isinstance(saved, torch.Tensor) else saved
 
     def __getstate__(self):
         raise RuntimeError("AdamW holds device buffers: save state_dict() instead of the optimizer")

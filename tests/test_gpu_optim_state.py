@@ -199,3 +199,56 @@ def test_a_negative_learning_rate_on_the_host_keeps_every_group_from_stepping():
         with pytest.raises((RuntimeError, ValueError), match="lr|learning rate"):
             opt.step()
     assert torch.equal(a, torch.ones_like(a)) and opt.moments[0].steps() == [0]
+
+
+# ---- checkpoints and the learning rate on the device ---------------------------------------------------------------------
+@pytest.mark.parametrize("loaded", ["host", "device", "number", "double"])
+def test_a_captured_step_follows_a_loaded_learning_rate(loaded):
+    """The loaded value goes into the scalar that the graph reads, wherever the checkpoint had it; schedulers go on from there."""
+    from superresolution_amd import optim
+
+    def build():
+        p = torch.nn.Parameter(_hash_floats(300, 1).cuda())
+        p.grad = _hash_floats(300, 2, 1e-2).cuda()
+        return p, torch.tensor(1e-3, device="cuda")
+    p, lr = build()
+    opt = optim.AdamW([p], lr=lr)
+    graph = _capture(opt.step)
+    graph.replay()
+    q, other = build()
+    ref = optim.AdamW([q], lr=other)
+    ref.step()
+    sd = opt.state_dict()
+    value = 0.25
+    sd["param_groups"][0]["lr"] = {"host": torch.tensor(value), "device": torch.tensor(value, device="cuda"), "number": value,
+                                   "double": torch.tensor(value, dtype=torch.float64, device="cuda")}[loaded]
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == value
+    other.fill_(value)
+    for k in range(3):
+        graph.replay()
+        ref.step()
+        assert torch.equal(p, q), k
+        for t in (opt.param_groups[0]["lr"], other):
+            t.mul_(0.5)
+
+
+def test_a_learning_rate_on_the_device_stays_there():
+    """Before anything is captured: a scalar of the optimizer's own, on its device, so that a later capture follows it."""
+    from superresolution_amd import optim
+    for value in (torch.tensor(0.25), 0.25, torch.tensor(0.25, dtype=torch.float64)):
+        p = torch.nn.Parameter(torch.ones(40, device="cuda"))
+        p.grad = torch.ones_like(p)
+        opt = optim.AdamW([p], lr=torch.tensor(1e-3, device="cuda"), weight_decay=0.0)
+        sd = opt.state_dict()
+        sd["param_groups"][0]["lr"] = value
+        opt.load_state_dict(sd)
+        lr = opt.param_groups[0]["lr"]
+        assert lr.is_cuda and lr.dtype == torch.float32 and float(lr) == 0.25 and lr is not value
+        graph = _capture(opt.step)
+        lr.zero_()
+        graph.replay()
+        assert torch.equal(p, torch.ones_like(p))
+        lr.fill_(0.5)
+        graph.replay()
+        assert (p < 1.0).all()
