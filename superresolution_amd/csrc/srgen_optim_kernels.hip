@@ -499,9 +499,9 @@ __device__ inline void adamw_chunk(const AdamWArgs& a, const Chunk& c, StepScala
             shared->c1 = (1.0 - sc.beta1) * f;
             shared->c2 = (1.0 - sc.beta2) * (f * f);
             shared->decay = (float)(1.0 - lr * sc.wd);
-            // (a step size of 0 or next to it: an infinite denominator, without infinity times a root that is 0; the reciprocal takes
-            // a subnormal for 0)
-            shared->ra = s == 0.0 ? 0.f : (float)fmin(1.0 / (s * sqrt(bc2)), 3.0e38);
+            // (a step size of 0 or next to it: an infinite denominator, by a finite factor that is not 0, so that neither a root of 0
+            // nor an infinite one makes NaN of it; the reciprocal takes a subnormal for 0)
+            shared->ra = (float)fmin(1.0 / (s * sqrt(bc2)), 3.0e38);
             shared->rb = s == 0.0 ? INFINITY : sc.eps == 0.0 ? 0.f : (float)fmax(sc.eps / s, 0x1p-126);
             shared->gmul = (float)f;
             shared->key = mix32(sc.seed_key + (uint32_t)t * kGold);

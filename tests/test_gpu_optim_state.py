@@ -252,3 +252,24 @@ def test_a_learning_rate_on_the_device_stays_there():
         lr.fill_(0.5)
         graph.replay()
         assert (p < 1.0).all()
+
+
+# ---- a step size of zero -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("on_device", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_learning_rate_of_zero_and_a_second_moment_that_overflows(bits, on_device):
+    """Gradients of 1e21: the second moment is infinite in 32 bits, the quotient 0 and the parameter where it was, as in torch."""
+    from superresolution_amd import optim
+    p, q = (torch.nn.Parameter(torch.ones(100, device="cuda")) for _ in range(2))
+    a = optim.AdamW([p], lr=torch.zeros((), device="cuda") if on_device else 0.0, state_bits=bits)
+    t = torch.optim.AdamW([q], lr=0.0)
+    for _ in range(2 if bits == 32 else 1):                              # (8 bits store it as NaN: the next step spoils the element)
+        for x in (p, q):
+            x.grad = torch.zeros_like(x)
+            x.grad[::3] = 1e21
+            x.grad[1::3] = 1e-3
+        a.step()
+        t.step()
+    assert torch.equal(p, q) and torch.equal(p, torch.ones_like(p))
+    if bits == 32:
+        assert torch.isinf(a.moments[0].exp_avg_sq[:100:3]).all()
