@@ -418,14 +418,20 @@ class AdamW(torch.optim.Optimizer):
             if len({id(p) for p in g["params"]}) != len(g["params"]):
                 raise ValueError("AdamW: a parameter appears twice in a group")
             self._check_memory()
-        except Exception:
+            # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
+            if self.max_grad_norm is not None and self._norm_fixed is None:
+                self._norm_fixed = torch.full((2,), -1.0, dtype=torch.float32, device=dev)      # (-1: nothing yet)
+            mo, ls = Moments([p.numel() for p in g["params"]], self.state_bits, dev), _Lists(g["params"])
+        except BaseException:
             self.param_groups.pop()
             raise
-        # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
-        self.moments.append(Moments([p.numel() for p in g["params"]], self.state_bits, dev))
-        self._lists.append(_Lists(g["params"]))
-        if self.max_grad_norm is not None and self._norm_fixed is None:
-            self._norm_fixed = torch.full((2,), -1.0, dtype=torch.float32, device=dev)      # (-1: nothing yet)
+        self.moments.append(mo)
+        self._lists.append(ls)
+
+    def _check_groups(self) -> None:
+        if len(self.param_groups) != len(self.moments):
+            raise RuntimeError(f"AdamW: {len(self.param_groups)} parameter groups, moments of {len(self.moments)}: groups come through "
+                               "add_param_group, and stay")
 
     @property
     def last_grad_norm(self) -> Optional[torch.Tensor]:
@@ -459,6 +465,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if len(self.param_groups) != len(self.moments):
+            self._check_groups()
         counts, kept = [], []
         for k, (group, mo, ls) in enumerate(zip(self.param_groups, self.moments, self._lists)):
             n = _tensorlist.params(group["params"], mo.device.index, mo._numel, ls.p, ls.p_code, ls.g, ls.g_code)
@@ -575,6 +583,7 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self) -> dict:
         """``torch.optim.AdamW.state_dict()``'s layout (``train.py:219-225`` saves it): fp32 moments and a step for each
         parameter that has taken one.  Reads the step counts back: one synchronisation."""
+        self._check_groups()
         state, groups, first = {}, [], 0
         for group, mo in zip(self.param_groups, self.moments):
             m, v = mo.read()
@@ -593,6 +602,7 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """Takes what ``state_dict`` (of this class, whatever its ``state_bits``, of ``torch.optim.AdamW`` or of
         ``training.FlatAdamW``) returns."""
+        self._check_groups()
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("loaded state dict contains a parameter group that doesn't match the size of optimizer's group")

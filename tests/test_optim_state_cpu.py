@@ -26,6 +26,37 @@ def _filled(optim, params, **kw):
     return opt
 
 
+def test_a_group_whose_moments_do_not_fit_is_not_added(optim, monkeypatch):
+    p, q = (torch.nn.Parameter(torch.ones(40)) for _ in range(2))
+    opt = optim.AdamW([p], lr=1e-2)
+
+    def full(*a):
+        raise torch.OutOfMemoryError("no memory for them")
+    monkeypatch.setattr(optim, "Moments", full)
+    with pytest.raises(torch.OutOfMemoryError):
+        opt.add_param_group(dict(params=[q]))
+    assert len(opt.param_groups) == len(opt.moments) == 1
+    monkeypatch.undo()
+    monkeypatch.setattr(optim, "_one_device", lambda ts, what: torch.device("cpu"))
+    opt.add_param_group(dict(params=[q]))                              # (and can be added afterwards)
+    assert len(opt.param_groups) == len(opt.moments) == 2
+
+
+@pytest.mark.parametrize("change", ["popped", "appended"])
+def test_groups_without_moments_of_their_own_are_refused(optim, change):
+    """A group put into the list, or taken out of it, by hand: the others would step with its moments, or it would not step."""
+    p, q = (torch.nn.Parameter(torch.ones(40)) for _ in range(2))
+    opt = _filled(optim, [dict(params=[p]), dict(params=[q])])
+    sd = opt.state_dict()
+    if change == "popped":
+        opt.param_groups.pop(0)
+    else:
+        opt.param_groups.append(dict(opt.param_groups[1], params=[torch.nn.Parameter(torch.ones(40))]))
+    for call in (opt.step, opt.state_dict, lambda: opt.load_state_dict(sd)):
+        with pytest.raises(RuntimeError, match="add_param_group"):
+            call()
+
+
 def test_tags_of_parameters_that_a_graph_writes():
     """A tag is the same again while nothing has written the tensor; never, where a replay may have, unseen by the host."""
     from superresolution_amd import versions
