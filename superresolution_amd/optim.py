@@ -583,6 +583,8 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self) -> dict:
         """``torch.optim.AdamW.state_dict()``'s layout (``train.py:219-225`` saves it): fp32 moments and a step for each
         parameter that has taken one.  Reads the step counts back: one synchronisation."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         self._check_groups()
         state, groups, first = {}, [], 0
         for group, mo in zip(self.param_groups, self.moments):
@@ -596,12 +598,20 @@ class AdamW(torch.optim.Optimizer):
                         torch.as_strided(x, p.shape, p.stride(), a)) for key, x in (("exp_avg", m), ("exp_avg_sq", v))}}
             groups.append({**{k: x for k, x in group.items() if k != "params"}, "params": list(range(first, first + len(group["params"])))})
             first += len(group["params"])
-        return {"state": state, "param_groups": groups}
+        sd = {"state": state, "param_groups": groups}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            given = hook(self, sd)
+            sd = sd if given is None else given
+        return sd
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
         """Takes what ``state_dict`` (of this class, whatever its ``state_bits``, of ``torch.optim.AdamW`` or of
         ``training.FlatAdamW``) returns."""
+        state_dict = state_dict.copy()
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            given = hook(self, state_dict)
+            state_dict = state_dict if given is None else given
         self._check_groups()
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
@@ -635,6 +645,8 @@ class AdamW(torch.optim.Optimizer):
             mo.write(m, v)
             lr = self._loaded_lr(group["lr"], saved.get("lr", group["lr"]))
             group.update({k: x.clone() if isinstance(x, torch.Tensor) else x for k, x in saved.items() if k not in ("params", "lr")}, lr=lr)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def _loaded_lr(self, lr, saved):
         """What a group's learning rate becomes: a scalar on the device stays one, and the very one that a captured step reads."""

@@ -57,6 +57,32 @@ def test_groups_without_moments_of_their_own_are_refused(optim, change):
             call()
 
 
+def test_state_dict_hooks_are_called(optim):
+    opt = _filled(optim, [torch.nn.Parameter(torch.ones(40))])
+    seen = []
+
+    def post(o, sd):
+        seen.append("post")
+        return {**sd, "extra": 7}
+    handles = [opt.register_state_dict_pre_hook(lambda o: seen.append("pre")), opt.register_state_dict_post_hook(post)]
+    sd = opt.state_dict()
+    assert seen == ["pre", "post"] and sd["extra"] == 7
+    for h in handles:
+        h.remove()
+    assert "extra" not in opt.state_dict() and len(seen) == 2
+
+    def rename(o, given):
+        seen.append("load pre")
+        return {"state": given["mine"], "param_groups": given["param_groups"]}
+    opt.register_load_state_dict_pre_hook(rename)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(o.moments[0].steps()))
+    given = {"mine": {0: {"step": torch.tensor(5.0), "exp_avg": torch.full((40,), 2.0), "exp_avg_sq": torch.ones(40)}},
+             "param_groups": sd["param_groups"]}
+    opt.load_state_dict(given)
+    assert seen[2:] == ["load pre", [5]] and set(given) == {"mine", "param_groups"}
+    assert torch.equal(opt.moments[0].exp_avg[:40], torch.full((40,), 2.0))
+
+
 def test_tags_of_parameters_that_a_graph_writes():
     """A tag is the same again while nothing has written the tensor; never, where a replay may have, unseen by the host."""
     from superresolution_amd import versions
