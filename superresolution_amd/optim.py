@@ -342,7 +342,8 @@ class _Lists:
         self.g_code = array("i", self.p_code)
         self.pg, self.codes = (_addr(self.p), _addr(self.g)), (_addr(self.p_code), _addr(self.g_code))
         self.checked = (array("Q"), array("i"))            # parameters' addresses and types that were last found apart
-        self.order = [_order(p) for p in params]           # of the parameters' memory, and so of their moments
+        self.shapes = [(p.shape, p.stride()) for p in params]          # as the moments have them
+        self.order = [_order(p) for p in params]
         self.plain = all(p.is_contiguous() for p in params)
 
 
@@ -580,6 +581,22 @@ class AdamW(torch.optim.Optimizer):
             ls.checked = ptr, code
 
     # -- checkpoints --------------------------------------------------------------------------------------------------
+    def _places(self, k: int) -> list:
+        """(shape, strides, offset) of each tensor of group ``k`` in the moments' buffers, by the order that the parameter was added
+        with; its present shape where that is the same memory."""
+        params, mo, ls = self.param_groups[k]["params"], self.moments[k], self._lists[k]
+        if list(map(_numel, params)) != mo.numels:
+            raise RuntimeError("AdamW: a parameter has another number of elements than when it was added")
+        places = []
+        for p, (shape, stride), offset in zip(params, ls.shapes, mo.offsets):
+            if p.shape != shape:
+                if not p.is_contiguous() or not ls.plain:
+                    raise RuntimeError(f"AdamW: a parameter of shape {tuple(p.shape)} and strides {p.stride()}: it was added with shape "
+                                       f"{tuple(shape)} and strides {stride}, which its moments still have")
+                shape, stride = p.shape, p.stride()
+            places.append((shape, stride, offset))
+        return places
+
     def state_dict(self) -> dict:
         """``torch.optim.AdamW.state_dict()``'s layout (``train.py:219-225`` saves it): fp32 moments and a step for each
         parameter that has taken one.  Reads the step counts back: one synchronisation."""
@@ -587,15 +604,13 @@ class AdamW(torch.optim.Optimizer):
             hook(self)
         self._check_groups()
         state, groups, first = {}, [], 0
-        for group, mo in zip(self.param_groups, self.moments):
+        for k, (group, mo) in enumerate(zip(self.param_groups, self.moments)):
             m, v = mo.read()
-            for i, (p, t) in enumerate(zip(group["params"], mo.steps())):
-                if t == 0:
-                    continue
-                a, n = mo.offsets[i], mo.numels[i]
-                state[first + i] = {"step": torch.tensor(float(t)), **{
-                    key: torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=mo.device).copy_(
-                        torch.as_strided(x, p.shape, p.stride(), a)) for key, x in (("exp_avg", m), ("exp_avg_sq", v))}}
+            for i, (p, t, place) in enumerate(zip(group["params"], mo.steps(), self._places(k))):
+                if t:
+                    state[first + i] = {"step": torch.tensor(float(t)), **{
+                        key: torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=mo.device).copy_(
+                            torch.as_strided(x, *place)) for key, x in (("exp_avg", m), ("exp_avg_sq", v))}}
             groups.append({**{k: x for k, x in group.items() if k != "params"}, "params": list(range(first, first + len(group["params"])))})
             first += len(group["params"])
         sd = {"state": state, "param_groups": groups}
@@ -627,17 +642,17 @@ class AdamW(torch.optim.Optimizer):
                     if key in state and state[key][name].numel() != p.numel():
                         raise ValueError(f"optimizer state of parameter {key} has {state[key][name].numel()} entries, the parameter {p.numel()}")
             _check_hyper({**group, **{k: x for k, x in saved.items() if k != "params"}})
-        for group, mo, saved in zip(self.param_groups, self.moments, groups):
+        for k, (group, mo, saved) in enumerate(zip(self.param_groups, self.moments, groups)):
             m = torch.zeros(mo.total, dtype=torch.float32, device=mo.device)
             v = torch.zeros_like(m)
             steps, into, values = [], [], []
-            for i, (p, key) in enumerate(zip(group["params"], saved["params"])):
+            for place, key in zip(self._places(k), saved["params"]):
                 st = state.get(key)
                 steps.append(0 if st is None else int(float(st["step"])))
                 if st is not None:
                     for x, name in ((m, "exp_avg"), (v, "exp_avg_sq")):
-                        into.append(torch.as_strided(x, p.shape, p.stride(), mo.offsets[i]))
-                        values.append(st[name].detach().reshape(p.shape))
+                        into.append(torch.as_strided(x, *place))
+                        values.append(st[name].detach().reshape(place[0]))
             if into:
                 torch._foreach_copy_(into, values)
             if steps:

@@ -83,6 +83,38 @@ def test_state_dict_hooks_are_called(optim):
     assert torch.equal(opt.moments[0].exp_avg[:40], torch.full((40,), 2.0))
 
 
+@pytest.mark.parametrize("first, then", [(torch.contiguous_format, torch.channels_last), (torch.channels_last, torch.contiguous_format)])
+def test_checkpoints_of_a_parameter_of_another_memory_order(optim, first, then):
+    """The moments keep the order that the parameter was added with; a checkpoint has them by element all the same."""
+    w = torch.randn(6, 5, 3, 3)
+    p = torch.nn.Parameter(w.clone(memory_format=first))
+    opt = _filled(optim, [p])
+    want = {k: v.clone() for k, v in opt.state_dict()["state"][0].items()}
+    p.data = p.data.contiguous(memory_format=then)
+    got = opt.state_dict()["state"][0]
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    before = opt.moments[0].exp_avg.clone()
+    opt.moments[0].exp_avg.zero_()
+    opt.load_state_dict(opt.state_dict() | {"state": {0: want}})
+    assert torch.equal(opt.moments[0].exp_avg[:270], before[:270])
+
+
+def test_checkpoints_of_a_parameter_of_another_size_are_refused(optim):
+    p, q = (torch.nn.Parameter(torch.ones(n)) for n in (40, 40))
+    opt = _filled(optim, [p, q])
+    sd = opt.state_dict()
+    p.data = torch.ones(64)                                             # (its padded part and the next tensor's first moments)
+    with pytest.raises(RuntimeError, match="number of elements"):
+        opt.state_dict()
+    with pytest.raises((RuntimeError, ValueError), match="number of elements|entries"):
+        opt.load_state_dict(sd)
+    p.data = torch.ones(5, 8)                                           # (another shape of the same memory)
+    assert torch.equal(opt.state_dict()["state"][0]["exp_avg"].view(-1), sd["state"][0]["exp_avg"])
+    opt.param_groups[0]["params"].pop()
+    with pytest.raises(RuntimeError, match="number of elements"):
+        opt.state_dict()
+
+
 def test_tags_of_parameters_that_a_graph_writes():
     """A tag is the same again while nothing has written the tensor; never, where a replay may have, unseen by the host."""
     from superresolution_amd import versions
