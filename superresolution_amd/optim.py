@@ -636,19 +636,20 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: no amsgrad variant")
         if not all(g.get("decoupled_weight_decay", True) for g in groups):
             raise ValueError("AdamW: no variant that adds the weight decay to the gradient")
-        for group, saved in zip(self.param_groups, groups):
-            for i, (p, key) in enumerate(zip(group["params"], saved["params"])):
+        plan = []                                          # (every group is looked at before the first is written)
+        for k, (group, saved) in enumerate(zip(self.param_groups, groups)):
+            for p, key in zip(group["params"], saved["params"]):
                 for name in ("exp_avg", "exp_avg_sq"):
                     if key in state and state[key][name].numel() != p.numel():
                         raise ValueError(f"optimizer state of parameter {key} has {state[key][name].numel()} entries, the parameter {p.numel()}")
             _check_hyper({**group, **{k: x for k, x in saved.items() if k != "params"}})
-        for k, (group, mo, saved) in enumerate(zip(self.param_groups, self.moments, groups)):
+            plan.append((self._places(k), [int(float(state[key]["step"])) if key in state else 0 for key in saved["params"]]))
+        for (group, mo, saved), (places, steps) in zip(zip(self.param_groups, self.moments, groups), plan):
             m = torch.zeros(mo.total, dtype=torch.float32, device=mo.device)
             v = torch.zeros_like(m)
-            steps, into, values = [], [], []
-            for place, key in zip(self._places(k), saved["params"]):
+            into, values = [], []
+            for place, key in zip(places, saved["params"]):
                 st = state.get(key)
-                steps.append(0 if st is None else int(float(st["step"])))
                 if st is not None:
                     for x, name in ((m, "exp_avg"), (v, "exp_avg_sq")):
                         into.append(torch.as_strided(x, *place))

@@ -115,6 +115,24 @@ def test_checkpoints_of_a_parameter_of_another_size_are_refused(optim):
         opt.state_dict()
 
 
+@pytest.mark.parametrize("break_it", [lambda st: st.pop("step"), lambda st: st.pop("exp_avg_sq"), lambda st: st.update(exp_avg=torch.ones(3)),
+                                      lambda st: st.update(step="three")])
+def test_a_checkpoint_that_is_refused_changes_nothing(optim, break_it):
+    opt = _filled(optim, [dict(params=[torch.nn.Parameter(torch.ones(40))]), dict(params=[torch.nn.Parameter(torch.ones(33))])])
+    sd = opt.state_dict()
+    for st in sd["state"].values():
+        st["exp_avg"] = st["exp_avg"] * 2.0
+        st["step"] = torch.tensor(9.0)
+    for g in sd["param_groups"]:
+        g["lr"] = 1.0
+    break_it(sd["state"][1])
+    kept = [mo.exp_avg.clone() for mo in opt.moments]
+    with pytest.raises((KeyError, ValueError)):
+        opt.load_state_dict(sd)
+    assert all(torch.equal(a, mo.exp_avg) and mo.steps() == [3] for a, mo in zip(kept, opt.moments))
+    assert [g["lr"] for g in opt.param_groups] == [1e-2, 1e-2]
+
+
 def test_tags_of_parameters_that_a_graph_writes():
     """A tag is the same again while nothing has written the tensor; never, where a replay may have, unseen by the host."""
     from superresolution_amd import versions
