@@ -267,7 +267,7 @@ class GanStep:
         self.opt_g = self.gen.optimizer
         self.ws = self.gen.ws
         self.d = discriminator
-        self.opt_d = FlatAdamW(discriminator.parameters(), lr=lr_d, state_bits=state_bits)
+        self.opt_d = FlatAdamW(discriminator.parameters(), lr=lr_d, state_bits=state_bits, seed=1)      # (other random bits than opt_g's)
         self.dgrad = DiscriminatorGrad(discriminator, self.ws)
         self.w_adv, self.w_pix, self.w_ssim = weight_adversarial, weight_pixel, weight_ssim
         self.clip, self.real_label, self.fake_label, self.group = grad_clip_norm, real_label, fake_label, group

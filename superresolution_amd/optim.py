@@ -361,6 +361,11 @@ def _in_order_of(p: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
     return torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=g.device).copy_(g)
 
 
+def group_seed(seed: int, group: int) -> int:
+    """The seed of a group's random bits: positions count from 0 in every group's moments, and equal ones would round alike."""
+    return (seed + group * 0x9E3779B9) & 0xFFFFFFFF
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` over separate tensors, a whole parameter group in one or a few launches.
 
@@ -371,7 +376,8 @@ class AdamW(torch.optim.Optimizer):
                         stochastically, so that a moving average goes on moving when its change is under half a step.
     ``max_grad_norm``   clips the gradients of all groups by their total norm inside ``step`` (the gradients themselves stay as
                         they are); the norm is left in ``last_grad_norm``.
-    ``seed``            of the stochastic rounding, which depends on it, the step and the element only.
+    ``seed``            of the stochastic rounding, which depends on it, the step, the group and the element only (optimizers that
+                        train side by side take seeds of their own, or elements at the same place round with the same bits).
 
     A bf16 parameter is rounded stochastically.  ``lr`` may be a 0-dim fp32 tensor on the parameters' device: a captured step
     then follows it, and ``load_state_dict`` writes into it (before a capture it makes a new one, as torch does).  Parameters keep the memory order that they were added with (``to(memory_format=...)`` comes before the
@@ -487,7 +493,7 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
                                "scaler.step(optimizer)")
         calls = []                                         # (all of them before the first: no group steps if another is refused)
-        for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
+        for k, (n, group, mo, ls) in enumerate(zip(counts, self.param_groups, self.moments, self._lists)):
             if not n:
                 continue
             lr, (b1, b2) = group["lr"], group["betas"]
@@ -503,7 +509,7 @@ class AdamW(torch.optim.Optimizer):
                 _check_hyper({**group, "lr": lr})
             calls.append((group, mo, ls, _lib.srgen_adamw_args(
                 lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, None, None if div is None else div.data_ptr(),
-                None if found is None else found.data_ptr(), None, None, mo.norm_bytes, self.max_grad_norm or 0.0, self.seed,
+                None if found is None else found.data_ptr(), None, None, mo.norm_bytes, self.max_grad_norm or 0.0, group_seed(self.seed, k),
                 1 if group["maximize"] else 0)))
         with _on(dev):
             stream, capturing = _stream(dev), _capturing()

@@ -273,3 +273,26 @@ def test_a_learning_rate_of_zero_and_a_second_moment_that_overflows(bits, on_dev
     assert torch.equal(p, q) and torch.equal(p, torch.ones_like(p))
     if bits == 32:
         assert torch.isinf(a.moments[0].exp_avg_sq[:100:3]).all()
+
+
+# ---- groups and their random bits ------------------------------------------------------------------------------------------
+def test_groups_round_with_bits_of_their_own():
+    """Two groups of equal parameters and gradients: each as the oracle with the group's seed, and not alike."""
+    from superresolution_amd import optim
+    n = 4097
+    ps = [torch.nn.Parameter(_hash_floats(n, 1).cuda()) for _ in range(2)]
+    opt = optim.AdamW([dict(params=[p]) for p in ps], lr=1e-2, state_bits=8, seed=5)
+    refs = [R.AdamWRef(_f64(p), bits=8, lr=1e-2, seed=optim.group_seed(5, k)) for k, p in enumerate(ps)]
+    for s in range(2):
+        g = _hash_floats(n, 20 + s, 1e-2).cuda()
+        for p in ps:
+            p.grad = g.clone()
+        opt.step()
+        for k, (p, ref) in enumerate(zip(ps, refs)):
+            class Holder:
+                moments = [opt.moments[k]]
+            _check(Holder, [p], [ref], [ref.step(_f64(g))])
+            ref.p = _f64(p)
+    a, b = (mo.exp_avg.view(torch.uint8) for mo in opt.moments)
+    assert 0.05 < float((a != b).float().mean())                        # (of the roundings about a third differ by chance)
+    assert np.isfinite(_f64(ps[0])).all()

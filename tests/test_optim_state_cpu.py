@@ -172,3 +172,16 @@ def test_modules_go_by_the_tags():
         del owner
         gc.collect()
         assert module._signature() == module._signature()
+
+
+def test_group_seeds_differ():
+    """Same-position elements of two groups round with bits of their own; the first group's are the seed's."""
+    from oracle import optim_ref as R
+    from superresolution_amd import optim
+    seeds = [optim.group_seed(5, k) for k in range(100)]
+    assert seeds[0] == 5 and len(set(seeds)) == 100 and all(0 <= s < 1 << 32 for s in seeds)
+    # 4,096 positions: equal bits by chance in 1 of 65,536 each, so that 8 or more of them have probability under 1e-14
+    bits = [R.random_bits(np.arange(4096), s, 1) for s in seeds[:4]]
+    for i in range(4):
+        for j in range(i):
+            assert all((x == y).sum() < 8 for x, y in zip(bits[i], bits[j]))
