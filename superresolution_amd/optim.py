@@ -49,7 +49,9 @@ BLOCK = 32            # SRGEN_OPT_BLOCK: elements that share one scale (8-bit mo
 CHUNK = 4096          # SRGEN_OPT_CHUNK: elements of one step counter
 
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(dev).cuda_stream without the object
-_capturing = torch.cuda.is_current_stream_capturing
+_capturing = torch._C._cuda_isCurrentStreamCapturing  # torch.cuda.is_current_stream_capturing()
+_current_device = torch._C._cuda_getDevice            # torch.cuda.current_device(), the runtime initialised
+_HERE = contextlib.nullcontext()
 _CODE = {torch.float32: _lib.SRGEN_F32, torch.bfloat16: _lib.SRGEN_BF16, torch.float16: _lib.SRGEN_F16}
 _TYPES = frozenset((torch.float32, torch.bfloat16))                  # of parameters and their gradients
 _dtype_of, _device_of = attrgetter("dtype"), attrgetter("device")
@@ -63,7 +65,7 @@ def _stream(dev: torch.device) -> int:
 
 def _on(dev: torch.device):
     """``dev`` as the current device, for a launch."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if _current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _up(n: int, to: int) -> int:
@@ -337,7 +339,8 @@ _GLOBAL_HOOKS = (_torch_optimizer._global_optimizer_pre_hooks, _torch_optimizer.
 class _Lists:
     """A group's addresses and type codes, as the kernels' list wants them; filled anew at every step."""
 
-    def __init__(self, params: List[torch.Tensor]):
+    def __init__(self, params: List[torch.Tensor], seed: int):
+        self.seed = seed
         self.p, self.g, self.p_code = _arrays(len(params))
         self.g_code = array("i", self.p_code)
         self.pg, self.codes = (_addr(self.p), _addr(self.g)), (_addr(self.p_code), _addr(self.g_code))
@@ -426,9 +429,10 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW: a parameter appears twice in a group")
             self._check_memory()
             # (allocated here and not at the first step: a first step inside a capture would put them into the graph's memory)
-            if self.max_grad_norm is not None and self._norm_fixed is None:
+            if self._norm_fixed is None:
                 self._norm_fixed = torch.full((2,), -1.0, dtype=torch.float32, device=dev)      # (-1: nothing yet)
-            mo, ls = Moments([p.numel() for p in g["params"]], self.state_bits, dev), _Lists(g["params"])
+            mo = Moments([p.numel() for p in g["params"]], self.state_bits, dev)
+            ls = _Lists(g["params"], group_seed(self.seed, len(self._lists)))
         except BaseException:
             self.param_groups.pop()
             raise
@@ -444,7 +448,7 @@ class AdamW(torch.optim.Optimizer):
     def last_grad_norm(self) -> Optional[torch.Tensor]:
         """The gradients' total norm at the last step that clipped, eager or replayed, before clipping (0-dim device tensor; NaN
         where a step has been captured and none has run)."""
-        if not self._captured or self._norm_fixed is None:
+        if not self._captured or self.max_grad_norm is None:
             return None if self._norm_coef is None else self._norm_coef[-2]
         # (a new tensor: the next step writes the buffer)
         norm = self._norm_fixed[0]
@@ -485,7 +489,7 @@ class AdamW(torch.optim.Optimizer):
         if not any(counts):
             return loss
         dev = self.moments[0].device
-        div, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        div, found = self.__dict__.get("grad_scale"), self.__dict__.get("found_inf")
         for t in (div, found):
             if t is not None and (t.device != dev or t.dtype != torch.float32 or t.numel() != 1):
                 raise RuntimeError(f"AdamW: grad_scale and found_inf are fp32 scalars on {dev}")
@@ -493,7 +497,7 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW(max_grad_norm=...) clips the gradients as they are: call scaler.unscale_(optimizer) before "
                                "scaler.step(optimizer)")
         calls = []                                         # (all of them before the first: no group steps if another is refused)
-        for k, (n, group, mo, ls) in enumerate(zip(counts, self.param_groups, self.moments, self._lists)):
+        for n, group, mo, ls in zip(counts, self.param_groups, self.moments, self._lists):
             if not n:
                 continue
             lr, (b1, b2) = group["lr"], group["betas"]
@@ -509,7 +513,7 @@ class AdamW(torch.optim.Optimizer):
                 _check_hyper({**group, "lr": lr})
             calls.append((group, mo, ls, _lib.srgen_adamw_args(
                 lr, b1, b2, group["eps"], group["weight_decay"], lr_dev, None, None if div is None else div.data_ptr(),
-                None if found is None else found.data_ptr(), None, None, mo.norm_bytes, self.max_grad_norm or 0.0, group_seed(self.seed, k),
+                None if found is None else found.data_ptr(), None, None, mo.norm_bytes, self.max_grad_norm or 0.0, ls.seed,
                 1 if group["maximize"] else 0)))
         with _on(dev):
             stream, capturing = _stream(dev), _capturing()
