@@ -325,7 +325,7 @@ __device__ inline NormCoef norm_coef_of(double sum, double max_norm)
 // A thread takes V elements at a time: 4, or 8 of bf16 with 8-bit moments, where the arithmetic is what takes the time and half
 // as many threads to a block of 32 make its scale cheaper (268M parameters: 540 -> 494 us).
 // What bounds it: memory (32 bits: 28 bytes an fp32 element, 268M in 1,305 us = 5.76 TB/s, vector units 19 % busy; 8 bits fp32: 16
-// bytes, 5.5 TB/s at 50 %), but for 8 bits with bf16 parameters (10 bytes and 56 vector instructions an element, 268M in 480 us = 5.66
+// bytes, 5.5 TB/s at 50 %), but for 8 bits with bf16 parameters (10 bytes and 56 vector instructions an element, 268M in 494 us = 5.50
 // TB/s at 97 % busy).  In cache (3.2M fp32, 32 bits) 16 us = 5.6 TB/s; a single workgroup 4.2 us, most of it the launch.
 struct StepScalars {
     double c1, c2;          // (1 - beta1) * c, (1 - beta2) * c^2
@@ -644,7 +644,7 @@ __device__ inline double sum_squares(const void* p, uint32_t n)
 }
 
 // Sums of squares in 64 bits, in a fixed order: one partial sum for each workgroup's elements.  One pass over the gradients, bound by
-// memory: 73M fp32 in 44.6 us = 6.5 TB/s, 66M bf16 in 26 to 30 us = 4.4 to 5.1 TB/s (16 KB to 64 KB a workgroup: at most 8,192 partial sums is the
+// memory: 89M fp32 in 55.5 us = 6.4 TB/s, 85M bf16 in 36 us = 4.7 TB/s (16 KB to 64 KB a workgroup: at most 8,192 partial sums is the
 // best of 1,024 to 32,768: 86, 67, 61, 57, 60, 71 us for 120M bf16 values in 500 tensors when they took three launches; 50 us in
 // two).  Eight loads in flight instead of four halve the occupancy (57 -> 60 us).
 template <bool NT>
@@ -717,7 +717,7 @@ __global__ __launch_bounds__(256) void scale_many_kernel(const OptTensors ts, co
 
 // ---- moments to 8 bits and back ----------------------------------------------------------------------------------------
 // To the nearest: the stochastic rounding's cut with half a step added; values that 8 bits hold come back as they are.  One pass, 10
-// bytes an element either way: 3.2M packed in 7.0 us (4.6 TB/s, the launch in it), 60M read back in 88 us = 6.9 TB/s.
+// bytes an element either way: 3.2M packed in 7.2 us (4.5 TB/s, the launch in it), 60M read back in 87 us = 6.9 TB/s.
 __global__ __launch_bounds__(256) void moments_pack_kernel(const float* __restrict__ m, const float* __restrict__ v, uint64_t n,
                                                            uint8_t* __restrict__ m8, uint8_t* __restrict__ me, uint8_t* __restrict__ r8,
                                                            uint8_t* __restrict__ re)
