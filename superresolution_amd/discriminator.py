@@ -87,7 +87,7 @@ class Discriminator(nn.Module):
 
     # ---- HIP handle / weights ----------------------------------------------------------
     def _signature(self) -> Tuple:
-        return tuple(map(versions.tag, self.state_dict(keep_vars=True).values()))
+        return versions.tags(self.state_dict(keep_vars=True).values())
 
     def _handle(self, idx: int) -> int:
         L = _lib.lib()

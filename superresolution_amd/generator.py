@@ -98,7 +98,7 @@ class Generator(nn.Module):
     def _signature(self) -> Tuple:
         """(parameters, buffers): the train-mode forward reads no BatchNorm running statistics, so its own
         updates of those buffers must not force a re-upload before the next train-mode call."""
-        return tuple(map(versions.tag, self.parameters())), tuple(map(versions.tag, self.buffers()))
+        return versions.tags(self.parameters()), versions.tags(self.buffers())
 
     def _handle(self, device: torch.device, train: bool = False) -> int:
         idx = device.index if device.index is not None else torch.cuda.current_device()

@@ -31,6 +31,11 @@ def tag(t: torch.Tensor) -> tuple:
     return t.data_ptr(), t._version
 
 
+def tags(tensors) -> tuple:
+    """The tags of ``tensors``."""
+    return tuple(map(tag, tensors)) if _noted else tuple((t.data_ptr(), t._version) for t in tensors)
+
+
 def refuse_capture(what: str, device: int) -> None:
     """For an upload of weights through the host, which no graph would replay."""
     with torch.cuda.device(device):
