@@ -654,6 +654,14 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f"optimizer state of parameter {key} has {state[key][name].numel()} entries, the parameter {p.numel()}")
             _check_hyper({**group, **{k: x for k, x in saved.items() if k != "params"}})
             plan.append((self._places(k), [int(float(state[key]["step"])) if key in state else 0 for key in saved["params"]]))
+        if self._captured:
+            shared = {}                                    # scalars that are written in place
+            for group, saved in zip(self.param_groups, groups):
+                lr, value = group["lr"], saved.get("lr", group["lr"])
+                if isinstance(lr, torch.Tensor) and lr.is_cuda:
+                    value = torch.as_tensor(value).to(lr).reshape(())
+                    if not torch.equal(shared.setdefault(lr.data_ptr(), value), value):
+                        raise ValueError("AdamW: groups share a learning rate that a captured step reads, and the checkpoint has two for it")
         for (group, mo, saved), (places, steps) in zip(zip(self.param_groups, self.moments, groups), plan):
             m = torch.zeros(mo.total, dtype=torch.float32, device=mo.device)
             v = torch.zeros_like(m)

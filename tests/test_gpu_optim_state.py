@@ -254,6 +254,30 @@ def test_a_learning_rate_on_the_device_stays_there():
         assert (p < 1.0).all()
 
 
+def test_groups_that_share_a_captured_learning_rate():
+    """One scalar cannot take two values: such a checkpoint is refused, and nothing of it is loaded."""
+    from superresolution_amd import optim
+    ps = [torch.nn.Parameter(torch.ones(40, device="cuda")) for _ in range(2)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    lr = torch.tensor(1e-3, device="cuda")
+    opt = optim.AdamW([dict(params=[p]) for p in ps], lr=lr)
+    graph = _capture(opt.step)
+    graph.replay()
+    sd = opt.state_dict()
+    sd["param_groups"][0]["lr"], sd["param_groups"][1]["lr"] = 0.25, 0.5
+    for st in sd["state"].values():
+        st["exp_avg"] = st["exp_avg"] * 2.0
+    kept = [mo.exp_avg.clone() for mo in opt.moments]
+    with pytest.raises(ValueError, match="share"):
+        opt.load_state_dict(sd)
+    assert float(lr) == float(torch.tensor(1e-3)) and all(torch.equal(a, mo.exp_avg) for a, mo in zip(kept, opt.moments))
+    sd["param_groups"][1]["lr"] = torch.tensor(0.25, dtype=torch.float64)
+    opt.load_state_dict(sd)
+    assert float(lr) == 0.25 and all(g["lr"] is lr for g in opt.param_groups)
+    assert all(torch.equal(2.0 * a, mo.exp_avg) for a, mo in zip(kept, opt.moments))
+
+
 # ---- a step size of zero -------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("on_device", [False, True])
 @pytest.mark.parametrize("bits", [32, 8])
