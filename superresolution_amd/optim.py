@@ -621,7 +621,8 @@ class AdamW(torch.optim.Optimizer):
                     state[first + i] = {"step": torch.tensor(float(t)), **{
                         key: torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=mo.device).copy_(
                             torch.as_strided(x, *place)) for key, x in (("exp_avg", m), ("exp_avg_sq", v))}}
-            groups.append({**{k: x for k, x in group.items() if k != "params"}, "params": list(range(first, first + len(group["params"])))})
+            groups.append({**{k: x.detach().clone() if isinstance(x, torch.Tensor) else x for k, x in group.items() if k != "params"},
+                           "params": list(range(first, first + len(group["params"])))})
             first += len(group["params"])
         sd = {"state": state, "param_groups": groups}
         for hook in self._optimizer_state_dict_post_hooks.values():

@@ -278,6 +278,20 @@ def test_groups_that_share_a_captured_learning_rate():
     assert all(torch.equal(2.0 * a, mo.exp_avg) for a, mo in zip(kept, opt.moments))
 
 
+def test_a_state_dict_keeps_its_learning_rate():
+    """Like the moments beside it, the learning rate of a checkpoint in memory is that of the moment it was taken."""
+    from superresolution_amd import optim
+    p = torch.nn.Parameter(torch.ones(40, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = optim.AdamW([p], lr=torch.tensor(0.25, device="cuda"))
+    graph = _capture(opt.step)
+    graph.replay()
+    sd = opt.state_dict()
+    opt.param_groups[0]["lr"].fill_(1.0)
+    opt.load_state_dict(sd)
+    assert float(opt.param_groups[0]["lr"]) == 0.25
+
+
 # ---- a step size of zero -------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("on_device", [False, True])
 @pytest.mark.parametrize("bits", [32, 8])
