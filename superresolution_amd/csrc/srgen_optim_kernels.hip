@@ -325,8 +325,8 @@ __device__ inline NormCoef norm_coef_of(double sum, double max_norm)
 // A thread takes V elements at a time: 4, or 8 of bf16 with 8-bit moments, where the arithmetic is what takes the time and half
 // as many threads to a block of 32 make its scale cheaper (268M parameters: 540 -> 494 us).
 // What bounds it: memory (32 bits: 28 bytes an fp32 element, 268M in 1,305 us = 5.76 TB/s, vector units 19 % busy; 8 bits fp32: 16
-// bytes, 5.5 TB/s at 50 %), but for 8 bits with bf16 parameters (10 bytes and 56 vector instructions an element, 268M in 494 us = 5.50
-// TB/s at 97 % busy).  In cache (3.2M fp32, 32 bits) 16 us = 5.6 TB/s; a single workgroup 4.2 us, most of it the launch.
+// bytes, 5.5 TB/s at 50 %), but for 8 bits with bf16 parameters (10 bytes and 56 vector instructions an element, 268M in 479 to 494 us,
+// by the card, = 5.5 to 5.7 TB/s at 97 % busy).  In cache (3.2M fp32, 32 bits) 16 us = 5.6 TB/s; a single workgroup 4.2 us, most of it the launch.
 struct StepScalars {
     double c1, c2;          // (1 - beta1) * c, (1 - beta2) * c^2
     float decay;            // 1 - lr wd

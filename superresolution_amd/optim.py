@@ -383,8 +383,8 @@ class AdamW(torch.optim.Optimizer):
                         train side by side take seeds of their own, or elements at the same place round with the same bits).
 
     A bf16 parameter is rounded stochastically.  ``lr`` may be a 0-dim fp32 tensor on the parameters' device: a captured step
-    then follows it, and ``load_state_dict`` writes into it (before a capture it makes a new one, as torch does).  Parameters keep the memory order that they were added with (``to(memory_format=...)`` comes before the
-    optimizer).  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
+    then follows it, and ``load_state_dict`` writes into it (before a capture it makes a new one, as torch does).  Parameters keep
+    the memory order that they were added with (``to(memory_format=...)`` comes before the optimizer).  ``step`` can be captured into a graph (the step counts are on the device); parameters, gradients and the
     optimizer have to stay.  While it does, ``Generator`` and ``Discriminator`` take its parameters for changed at every use (a replay
     raises no version counter, ``versions``).  ``torch.amp.GradScaler`` hands its scale and its flag to ``step``: a step with a non-finite
     gradient does not happen.  ``state_dict`` has the layout of ``torch.optim.AdamW`` with fp32 moments, whatever
